@@ -297,6 +297,100 @@ TRMOE_API int tr_gpu_attn_decode(tr_gpu_attn *a, int64_t layer, int64_t pos, con
 TRMOE_API int tr_gpu_attn_warm(tr_gpu_attn *a, uint64_t ns);
 
 /* ---------------------------------------------------------------------------------------------
+ * Attention over a KV cache in 4 bits. No counterpart in the reference (its caches hold f32): for engines that keep
+ * their activations on the GPU, serve several sequences, share KV heads between query heads, or need contexts that
+ * f32 keys and values leave no room for (6.4 times smaller: 16 layers, 16 heads of 128 and 4096 positions are
+ * 0.17 GB instead of 1.07). Results are not the reference's bits: keys and values are quantised.
+ *
+ * A session holds, per layer, n_seq sequences ("slots") of n_ctx positions. A row (one position's key or value of one
+ * KV head) is held in groups of 32 values, 5 bits a value: per group a minimum m = f16(min) and a scale
+ * d = f16(max(0, max - m) / 15), per value the code clamp(rint((x - m) / d), 0, 15) (0 where d is 0); it stands for
+ * f32(m + d code). Every rounding is to nearest even of the real value. A group with a NaN or an infinity, or whose m
+ * or d passes f16, reads back as NaN.
+ *
+ * The device calls enqueue on `stream` (a cudaStream_t; NULL: the default stream), never wait and allocate nothing, so a
+ * CUDA graph can hold them. They share no workspace: calls of one session may overlap on several streams as long as
+ * none writes what another one of them reads or writes (the caller orders those). Each makes the session's device
+ * current on the calling thread; every pointer is memory of that device, rows of `type` (TRMOE_F32, TRMOE_F16 or
+ * TRMOE_BF16), a row's heads side by side, strides in values between rows; rows start on 16-byte boundaries (the
+ * stride too) and must not overlap in an output. 0, or -1 with trmoe_last_error(). */
+typedef struct tr_gpu_attn4 tr_gpu_attn4;
+#define TRMOE_ATTN4_BLOCK 64      /* positions of a selectable block */
+#define TRMOE_ATTN4_MAX_GROUP 256 /* query heads a KV head */
+
+typedef struct {
+    int64_t n_layers;  /* layers held */
+    int64_t n_seq;     /* sequences a layer holds (<= 65535) */
+    int64_t n_head;    /* query heads, a multiple of n_kv_head (query head h reads KV head h / (n_head / n_kv_head)) */
+    int64_t n_kv_head;
+    int64_t head_dim;  /* 64 or 128 */
+    int64_t n_ctx;     /* positions a sequence has room for (<= 2^24) */
+} tr_gpu_attn4_config;
+
+/* Which rows of a call belong where. The arrays are device memory (a captured call reads them when it is replayed).
+ * Entry i holds the call's rows start[i] .. start[i + 1] - 1, which are at positions pos0[i], pos0[i] + 1, .. of
+ * sequence slot[i]. A negative slot is padding: its rows are neither read nor written, and so are rows that belong to
+ * no entry. An entry whose slot, positions or rows pass the session, n_tok or max_rows is left out the same way, and
+ * tr_gpu_attn4_check says so. */
+typedef struct {
+    int64_t n_entries;    /* <= 65535 */
+    int64_t n_tok;        /* rows of the call's arrays */
+    int64_t max_rows;     /* at least the most rows of an entry (at most n_ctx); sizes the launch. Not read without start */
+    const int32_t *slot;  /* [n_entries] */
+    const int32_t *pos0;  /* [n_entries] */
+    const int32_t *start; /* [n_entries + 1], or NULL: one row an entry (n_tok = n_entries) */
+} tr_gpu_attn4_batch;
+
+/* A session on the device of g (which must outlive it), its cache zero. NULL with a message when the shape is not
+ * supported or HBM would keep less than TRMOE_GPU_VRAM_RESERVE free. */
+TRMOE_API tr_gpu_attn4 *tr_gpu_attn4_create(tr_gpu *g, const tr_gpu_attn4_config *cfg, char *err, size_t err_len);
+/* NULL: nothing. The caller's work on the session must have finished. */
+TRMOE_API void tr_gpu_attn4_free(tr_gpu_attn4 *a);
+/* The HBM a session of that shape takes (0: not supported). */
+TRMOE_API uint64_t tr_gpu_attn4_bytes(const tr_gpu_attn4_config *cfg);
+
+/* Quantises the rows k and v [n_tok][n_kv_head * head_dim] into their positions, and keeps the bounds that
+ * tr_gpu_attn4_select_dev scores the touched blocks by. Entries of one call name different slots: a slot named again
+ * is left out of the later entry, and tr_gpu_attn4_check says so. */
+TRMOE_API int tr_gpu_attn4_write_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type,
+                                     const void *k, int64_t k_stride, const void *v, int64_t v_stride, void *stream);
+/* The values that the batch's positions stand for, into k and v [n_tok][n_kv_head * head_dim] (a position never
+ * written: 0). */
+TRMOE_API int tr_gpu_attn4_read_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type, void *k,
+                                    int64_t k_stride, void *v, int64_t v_stride, void *stream);
+/* out row = softmax(scale q.k) v over positions 0 .. p of the row's sequence, p the row's own position (whose key and
+ * value a write has stored before): one row an entry is a decode step, several are a prompt or drafted tokens. q and
+ * out [n_tok][n_head * head_dim]. Scores, softmax and sums are in 32 bits. */
+TRMOE_API int tr_gpu_attn4_attend_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type,
+                                      const void *q, int64_t q_stride, float scale, void *out, int64_t out_stride,
+                                      void *stream);
+/* tr_gpu_attn4_attend_dev over n_blocks blocks of TRMOE_ATTN4_BLOCK positions (1 to 4096) for each row and KV head: the
+ * block of the row's own position, up to it, and the n_blocks - 1 earlier ones of the highest score, ties to the lowest
+ * index (all of them when there are no more). A block's score is an upper bound of its keys' summed q.k over the KV
+ * head's query heads, in whole numbers: f32(sum_i P_i hi_i + N_i lo_i) * unit, where
+ *   unit = 2^(e-7) with 2^(e-1) <= the largest |value| of the block's 64 keys < 2^e (2^-7 where that is 0), and
+ *   lo_i, hi_i = floor and ceil of dim i's lowest and highest value / unit, within -127 .. 127;
+ *   P_i, N_i = the sums over the query heads of max(z, 0) and min(z, 0), z = rint(q_i / u) within -127 .. 127, and u
+ *   made of the query heads' largest |q_i| like the unit.
+ * A block with a NaN among its keys scores +infinity; a row with a NaN or an infinity in q has P = N = 0. blocks
+ * (optional): [n_tok][n_kv_head][n_blocks] int32, the blocks attended to in increasing order, then -1. */
+TRMOE_API int tr_gpu_attn4_select_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type,
+                                      const void *q, int64_t q_stride, float scale, int64_t n_blocks, void *out,
+                                      int64_t out_stride, int32_t *blocks, void *stream);
+/* Waits for the session's device and reports whether a call since the last check left an entry out (see
+ * tr_gpu_attn4_batch and tr_gpu_attn4_write_dev) or gave up on a bounded wait; then cleared. 0, or -1 with a message. */
+TRMOE_API int tr_gpu_attn4_check(tr_gpu_attn4 *a);
+
+/* tr_gpu_attn_write and tr_gpu_attn_decode (above) over the 4-bit cache, for engines with host rows: the same
+ * arguments, with the sequence's slot; k and v [n_tok][n_kv_head * head_dim], q and out [n_head * head_dim], f32. They
+ * run on the session's own stream, which the default stream orders itself with, and return when it has finished; work
+ * that the caller put on other streams must have finished before. One thread at a time. */
+TRMOE_API int tr_gpu_attn4_write(tr_gpu_attn4 *a, int64_t layer, int64_t slot, int64_t pos0, int64_t n_tok,
+                                 const float *k, const float *v);
+TRMOE_API int tr_gpu_attn4_decode(tr_gpu_attn4 *a, int64_t layer, int64_t slot, int64_t pos, const float *q,
+                                  const float *k, const float *v, float scale, float *out);
+
+/* ---------------------------------------------------------------------------------------------
  * 2. The kernel level (Trochilus src/kernels/kernels.h) */
 
 typedef struct tr_pool tr_pool; /* the reference's thread pool: accepted and ignored */

@@ -14,8 +14,10 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
+#include <type_traits>
 #include <unordered_map>
 #include <vector>
 
@@ -29,6 +31,7 @@
 #include "decode.cuh"
 #include "gguf_file.h"
 #include "attention.cuh"
+#include "attention4.cuh"
 #include "prefill.cuh"
 #include "ep.cuh"
 #include "ffn_norm.cuh"
@@ -1320,5 +1323,7 @@ extern "C" int tr_gpu_moe_ffn_dev(tr_gpu_moe *m, int64_t layer, int64_t n_tok, f
 #include "capi_ep.inc"
 
 #include "capi_attention.inc"
+
+#include "capi_attention4.inc"
 
 #include "capi_kernel_level.inc"

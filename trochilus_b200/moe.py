@@ -34,7 +34,9 @@ EXPORTS = ["tr_gpu_moe_create", "tr_gpu_moe_free", "tr_gpu_moe_bytes", "tr_gpu_m
            "tr_matmul_q4x_prepared_n", "tr_q4x_fused_calls", "tr_swiglu_prepare", "tr_gpu_moe_config_from_gguf",
            "tr_gpu_moe_load_gguf", "tr_gpu_open", "tr_gpu_close", "tr_gpu_name", "tr_gpu_attn_create",
            "tr_gpu_attn_free", "tr_gpu_attn_bytes", "tr_gpu_attn_write", "tr_gpu_attn_decode", "tr_gpu_attn_warm",
-           "trmoe_kernel_arch"]
+           "tr_gpu_attn4_create", "tr_gpu_attn4_free", "tr_gpu_attn4_bytes", "tr_gpu_attn4_write_dev",
+           "tr_gpu_attn4_read_dev", "tr_gpu_attn4_attend_dev", "tr_gpu_attn4_select_dev", "tr_gpu_attn4_check",
+           "tr_gpu_attn4_write", "tr_gpu_attn4_decode", "trmoe_kernel_arch"]
 
 
 class Config(C.Structure):
@@ -50,6 +52,17 @@ class Outputs(C.Structure):
 
 class TrMat(C.Structure):
     _fields_ = [("type", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64), ("data", C.c_void_p)]
+
+
+class Attn4Config(C.Structure):
+    _fields_ = [("n_layers", C.c_int64), ("n_seq", C.c_int64), ("n_head", C.c_int64), ("n_kv_head", C.c_int64),
+                ("head_dim", C.c_int64), ("n_ctx", C.c_int64)]
+
+
+class Attn4Batch(C.Structure):
+    """tr_gpu_attn4_batch: slot, pos0 and start are device pointers to int32 (start None: one row an entry)"""
+    _fields_ = [("n_entries", C.c_int64), ("n_tok", C.c_int64), ("max_rows", C.c_int64), ("slot", C.c_void_p),
+                ("pos0", C.c_void_p), ("start", C.c_void_p)]
 
 
 _lib = None
@@ -137,6 +150,20 @@ def lib():
     L.tr_gpu_attn_decode.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
                                      C.c_float, C.c_void_p]
     L.tr_gpu_attn_warm.argtypes = [C.c_void_p, C.c_uint64]
+    L.tr_gpu_attn4_create.restype = C.c_void_p
+    L.tr_gpu_attn4_create.argtypes = [C.c_void_p, C.POINTER(Attn4Config), C.c_char_p, C.c_size_t]
+    L.tr_gpu_attn4_free.argtypes = [C.c_void_p]
+    L.tr_gpu_attn4_bytes.restype = C.c_uint64
+    L.tr_gpu_attn4_bytes.argtypes = [C.POINTER(Attn4Config)]
+    rows = [C.c_void_p, C.c_int64, C.POINTER(Attn4Batch), C.c_int, C.c_void_p, C.c_int64]
+    L.tr_gpu_attn4_write_dev.argtypes = [*rows, C.c_void_p, C.c_int64, C.c_void_p]
+    L.tr_gpu_attn4_read_dev.argtypes = [*rows, C.c_void_p, C.c_int64, C.c_void_p]
+    L.tr_gpu_attn4_attend_dev.argtypes = [*rows, C.c_float, C.c_void_p, C.c_int64, C.c_void_p]
+    L.tr_gpu_attn4_select_dev.argtypes = [*rows, C.c_float, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
+    L.tr_gpu_attn4_check.argtypes = [C.c_void_p]
+    L.tr_gpu_attn4_write.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]
+    L.tr_gpu_attn4_decode.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.c_float, C.c_void_p]
     _lib = L
     return L
 
@@ -416,6 +443,94 @@ class GpuAttn:
     def close(self):
         if getattr(self, "a", None):
             lib().tr_gpu_attn_free(self.a)
+            self.a = None
+        if getattr(self, "g", None):
+            lib().tr_gpu_close(self.g)
+            self.g = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class GpuAttn4:
+    """A tr_gpu_attn4 session: n_layers layers of n_seq sequences of n_ctx positions, keys and values held in 4 bits.
+    The *_dev calls take device pointers (e.g. torch tensors' data_ptr()) and an Attn4Batch, and are enqueued on
+    `stream` (0: the default stream); type is F32, F16 or BF16, strides are in values."""
+
+    def __init__(self, n_layers: int, n_seq: int, n_head: int, n_kv_head: int, head_dim: int, n_ctx: int):
+        L = lib()
+        self.cfg = Attn4Config(n_layers, n_seq, n_head, n_kv_head, head_dim, n_ctx)
+        err = C.create_string_buffer(512)
+        self.g = L.tr_gpu_open(err, 512)
+        if not self.g:
+            raise RuntimeError(f"tr_gpu_open: {err.value.decode()}")
+        self.a = L.tr_gpu_attn4_create(self.g, C.byref(self.cfg), err, 512)
+        if not self.a:
+            L.tr_gpu_close(self.g)
+            self.g = None
+            raise RuntimeError(f"tr_gpu_attn4_create: {err.value.decode()}")
+
+    @staticmethod
+    def bytes_needed(n_layers: int, n_seq: int, n_head: int, n_kv_head: int, head_dim: int, n_ctx: int) -> int:
+        return int(lib().tr_gpu_attn4_bytes(C.byref(Attn4Config(n_layers, n_seq, n_head, n_kv_head, head_dim, n_ctx))))
+
+    def write_dev(self, layer: int, batch: Attn4Batch, type_: int, k_ptr: int, k_stride: int, v_ptr: int, v_stride: int,
+                  stream: int = 0):
+        """tr_gpu_attn4_write_dev: k and v rows of n_kv_head * head_dim into the batch's positions"""
+        if _lib.tr_gpu_attn4_write_dev(self.a, layer, batch, type_, k_ptr, k_stride, v_ptr, v_stride, stream) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_write_dev: {last_error()}")
+
+    def read_dev(self, layer: int, batch: Attn4Batch, type_: int, k_ptr: int, k_stride: int, v_ptr: int, v_stride: int,
+                 stream: int = 0):
+        """tr_gpu_attn4_read_dev: what the batch's positions hold, into k and v rows"""
+        if _lib.tr_gpu_attn4_read_dev(self.a, layer, batch, type_, k_ptr, k_stride, v_ptr, v_stride, stream) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_read_dev: {last_error()}")
+
+    def attend_dev(self, layer: int, batch: Attn4Batch, type_: int, q_ptr: int, q_stride: int, scale: float,
+                   out_ptr: int, out_stride: int, stream: int = 0):
+        """tr_gpu_attn4_attend_dev: q and out rows of n_head * head_dim; each row attends up to its own position"""
+        if _lib.tr_gpu_attn4_attend_dev(self.a, layer, batch, type_, q_ptr, q_stride, scale, out_ptr, out_stride,
+                                        stream) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_attend_dev: {last_error()}")
+
+    def select_dev(self, layer: int, batch: Attn4Batch, type_: int, q_ptr: int, q_stride: int, scale: float,
+                   n_blocks: int, out_ptr: int, out_stride: int, blocks_ptr: int | None = None, stream: int = 0):
+        """tr_gpu_attn4_select_dev: attend_dev over the n_blocks blocks of 64 positions that each row's scores select;
+        blocks_ptr (optional): int32 [n_tok][n_kv_head][n_blocks]"""
+        if _lib.tr_gpu_attn4_select_dev(self.a, layer, batch, type_, q_ptr, q_stride, scale, n_blocks, out_ptr,
+                                        out_stride, blocks_ptr, stream) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_select_dev: {last_error()}")
+
+    def check(self):
+        """tr_gpu_attn4_check: wait for the device; raise if a call left an entry out"""
+        if lib().tr_gpu_attn4_check(self.a) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_check: {last_error()}")
+
+    def write(self, layer: int, slot: int, pos0: int, k: np.ndarray, v: np.ndarray):
+        """tr_gpu_attn4_write on host arrays: k, v [n_tok][n_kv_head * head_dim]"""
+        row = self.cfg.n_kv_head * self.cfg.head_dim
+        k = np.ascontiguousarray(k, dtype=np.float32).reshape(-1, row)
+        v = np.ascontiguousarray(v, dtype=np.float32).reshape(-1, row)
+        assert k.shape == v.shape
+        if lib().tr_gpu_attn4_write(self.a, layer, slot, pos0, k.shape[0], _p(k), _p(v)) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_write: {last_error()}")
+
+    def decode(self, layer: int, slot: int, pos: int, q, k, v, scale: float) -> np.ndarray:
+        """tr_gpu_attn4_decode on host arrays: q [n_head * head_dim], k and v [n_kv_head * head_dim]; returns out
+        [n_head][head_dim]"""
+        q, k, v = (np.ascontiguousarray(a, dtype=np.float32).ravel() for a in (q, k, v))
+        assert q.size == self.cfg.n_head * self.cfg.head_dim and k.size == v.size == self.cfg.n_kv_head * self.cfg.head_dim
+        out = np.full((self.cfg.n_head, self.cfg.head_dim), np.nan, dtype=np.float32)
+        if lib().tr_gpu_attn4_decode(self.a, layer, slot, pos, _p(q), _p(k), _p(v), scale, _p(out)) != 0:
+            raise RuntimeError(f"tr_gpu_attn4_decode: {last_error()}")
+        return out
+
+    def close(self):
+        if getattr(self, "a", None):
+            lib().tr_gpu_attn4_free(self.a)
             self.a = None
         if getattr(self, "g", None):
             lib().tr_gpu_close(self.g)
