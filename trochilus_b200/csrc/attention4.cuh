@@ -8,15 +8,17 @@
 // not depend on how they are computed. A group that holds a NaN or an infinity, or whose m or d passes f16, keeps
 // d = NaN, m = 0 and codes 0: it reads back as NaN, and m is always finite.
 //
-// 64 positions of a (layer, sequence, KV head) are one record of contiguous memory (10240 bytes for HD 128: 5 bits a
+// 32 positions of a (layer, sequence, KV head) are one record of contiguous memory (5120 bytes for HD 128: 5 bits a
 // value), one bulk copy of the attention kernel:
-//   keys    codes  [pos][c][g] one 32-bit word: dims 32 g + 8 c + j (j = 0..7) at bits 4 j        64 x HD / 2 bytes
-//           d      [pos / 2][g][pos % 2] f16, m [pos][g] f16
+//   keys    codes  [pos][c][g] one 32-bit word: dims 32 g + 8 c + j (j = 0..7) at bits 4 j        32 x HD / 2 bytes
+//           d, m   [pos][g] f16
 //   values  codes  [pos / 8][n][c][g][odd] 16 bits (pos % 8 = 2 c + odd): dims 32 g + 4 n + i (i = 0..3) at bits 4 i
 //           d, m   [pos / 2][g][pos % 2] f16
 // The words are what a lane of a tensor-core fragment takes (the attention kernel's comment): no two positions share
-// a byte of codes, so a position is written without reading its neighbours.
+// a byte of codes, so a position is written without reading its neighbours. Two records are a block of 64 positions,
+// the unit of selection.
 #pragma once
+#include <climits>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,18 +26,19 @@
 #include "bulk.cuh"
 #include "common.cuh"
 
-#define TRX_A4_BLOCK 64 // positions a record
+#define TRX_A4_REC 32   // positions a record
+#define TRX_A4_BLOCK 64 // positions a block
 
 template <int HD> struct TrxA4L { // byte offsets in a record
     static constexpr int NG = HD / 32;
-    static constexpr int KD = TRX_A4_BLOCK * HD / 2, KM = KD + TRX_A4_BLOCK * NG * 2;
-    static constexpr int V = KM + TRX_A4_BLOCK * NG * 2, VD = V + KD, VM = V + KM;
-    static constexpr int REC = 2 * V;
+    static constexpr int KD = TRX_A4_REC * HD / 2, KM = KD + TRX_A4_REC * NG * 2;
+    static constexpr int V = KM + TRX_A4_REC * NG * 2, VD = V + KD, VM = V + KM;
+    static constexpr int REC = 2 * V, BLOCK = 2 * REC;
 };
 
 struct TrxA4 { // one layer of a session
-    uint8_t *cache;  // [seq][KV head][block] records
-    int8_t *bounds;  // [seq][KV head][block][HD / 8]{lowest of 8 dims, highest of 8 dims}
+    uint8_t *cache;  // [seq][KV head][block] two records each
+    int8_t *bounds;  // [seq][KV head][block][2][HD]: lowest, then highest
     float *units;    // [seq][KV head][block]
     int32_t *err;
     int64_t n_ctx;
@@ -55,11 +58,11 @@ enum : int { TRX_A4_BAD_ENTRY = 1, TRX_A4_SAME_SLOT = 2, TRX_A4_GAVE_UP = 3 };
 __device__ __forceinline__ bool trx_a4_entry(const TrxA4 &a, const TrxA4Batch &b, int i, int &slot, int &row0,
                                              int &rows, int &pos0) {
     slot = b.slot[i];
-    if (slot < 0) return false;
+    pos0 = b.pos0[i];
     row0 = b.start ? b.start[i] : i;
     const int64_t r1 = b.start ? b.start[i + 1] : i + 1;
     const int64_t n = r1 - row0;
-    pos0 = b.pos0[i];
+    if (slot < 0) return false;
     if (slot >= a.n_seq || row0 < 0 || n < 0 || r1 > b.n_tok || n > b.max_rows || pos0 < 0 || pos0 + n > a.n_ctx) {
         atomicCAS(a.err, 0, TRX_A4_BAD_ENTRY);
         return false;
@@ -68,28 +71,39 @@ __device__ __forceinline__ bool trx_a4_entry(const TrxA4 &a, const TrxA4Batch &b
     return n > 0;
 }
 
-// 8 consecutive values of a row, as floats, and back
-__device__ __forceinline__ void trx_a4_load8(const float *p, float (&x)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+// 8 consecutive values of a row: as they lie in memory, as floats, and back
+template <typename T> struct TrxA4Raw {
+    uint4 w[sizeof(T) / 2];
+};
+template <typename T> __device__ __forceinline__ TrxA4Raw<T> trx_a4_raw8(const T *p) {
+    TrxA4Raw<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
 }
-__device__ __forceinline__ void trx_a4_load8(const __half *p, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void trx_a4_floats(const TrxA4Raw<float> &r, float (&x)[8]) {
+    const uint32_t u[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __uint_as_float(u[i]);
+}
+__device__ __forceinline__ void trx_a4_floats(const TrxA4Raw<__half> &r, float (&x)[8]) {
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
         x[2 * i] = f.x, x[2 * i + 1] = f.y;
     }
 }
-__device__ __forceinline__ void trx_a4_load8(const __nv_bfloat16 *p, float (&x)[8]) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void trx_a4_floats(const TrxA4Raw<__nv_bfloat16> &r, float (&x)[8]) {
+    const uint32_t u[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         x[2 * i] = __uint_as_float(u[i] << 16);
         x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
+}
+template <typename T> __device__ __forceinline__ void trx_a4_load8(const T *p, float (&x)[8]) {
+    trx_a4_floats(trx_a4_raw8(p), x);
 }
 __device__ __forceinline__ void trx_a4_store8(float *p, const float (&x)[8]) {
     reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -108,67 +122,104 @@ template <typename T> __device__ __forceinline__ void trx_a4_store8(T *p, const 
                                                trx_a4_pack2(x[4], x[5], p), trx_a4_pack2(x[6], x[7], p));
 }
 
+// three-operand minimum and maximum (a NaN beside a number is dropped)
+__device__ __forceinline__ float trx_a4_min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float trx_a4_max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // The 8 codes (4 bits each, value j at bits 4 j), scale and minimum of 8 values of a group whose other 24 lie in the
-// lanes next to this one (4 aligned lanes a group; the whole warp calls).
-// The quotient is taken in 32 bits, which is within 3 x 2^-24 x 22 < 4e-6 of the real one (a quotient is at most 15
-// plus m's and d's roundings, below 22 even where d is a subnormal); one within 1e-5 of a border is taken again in
-// 64 bits.
-__device__ __forceinline__ uint32_t trx_a4_quant(const float (&x)[8], uint16_t &d16, uint16_t &m16) {
-    float lo = x[0], hi = x[0];
-    bool bad = false;
+// lanes next to this one (4 aligned lanes a group; the whole warp calls); x becomes what they stand for.
+// Both are taken in 32 bits, and exactly where that may round to another side. (hi - m) / 15 is off by less than 2^-22 of
+// itself, so it is certain unless 1 - 2^-21 and 1 + 2^-21 times it round apart (then: in 64 bits). A quotient, kept within
+// 0 .. 15 as 15 times the saturated (x - m) / (15 d) (15 d is exact), is off by less than 4 x 2^-24 x 15 < 4e-6, so it is
+// certain unless it is within 2e-5 of a border. Then x is compared with the border m + (k + 1/2) d itself, whose second
+// term is exact: with its nearest float s, and where x is s, with what s dropped. (16-bit inputs meet such borders often.)
+__device__ __forceinline__ uint32_t trx_a4_quant(float (&x)[8], uint16_t &d16, uint16_t &m16) {
+    float lo = trx_a4_min3(x[0], x[1], x[2]), hi = trx_a4_max3(x[0], x[1], x[2]), none = 0.0f;
+    lo = trx_a4_min3(lo, x[3], x[4]), hi = trx_a4_max3(hi, x[3], x[4]);
+    lo = trx_a4_min3(lo, x[5], x[6]), hi = trx_a4_max3(hi, x[5], x[6]);
+    lo = fminf(lo, x[7]), hi = fmaxf(hi, x[7]);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        lo = fminf(lo, x[j]);
-        hi = fmaxf(hi, x[j]);
-        bad |= !(fabsf(x[j]) <= 3.402823466e38f);
-    }
+    for (int j = 0; j < 8; j++) none = __fmaf_rn(x[j], 0.0f, none); // (0, or NaN where a value is not finite)
 #pragma unroll
     for (int s = 1; s <= 2; s <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, s) != 0;
+        none += __shfl_xor_sync(0xffffffffu, none, s);
     }
     const __half mh = __float2half_rn(lo);
     const float m = __half2float(mh);
-    const __half dh = __double2half(__ddiv_rn(fmax(__dsub_rn((double)hi, (double)m), 0.0), 15.0));
+    const float step = __fmul_rn(fmaxf(__fsub_rn(hi, m), 0.0f), 0.0666666701f);
+    __half dh = __float2half_rn(__fmul_rn(step, 1.0f - 4.76837158e-7f));
+    if (__half_as_ushort(dh) != __half_as_ushort(__float2half_rn(__fmul_rn(step, 1.0f + 4.76837158e-7f))))
+        dh = __double2half(__ddiv_rn(fmax(__dsub_rn((double)hi, (double)m), 0.0), 15.0));
     const float d = __half2float(dh);
-    bad |= !(fabsf(m) <= 65504.0f) || !(d <= 65504.0f);
+    const bool bad = none != 0.0f || !(fabsf(m) <= 65504.0f) || !(d <= 65504.0f);
     d16 = bad ? (uint16_t)0x7fff : __half_as_ushort(dh);
     m16 = bad ? (uint16_t)0 : __half_as_ushort(mh);
-    if (bad || d == 0.0f) return 0;
-    const float rd = __fdiv_rn(1.0f, d);
-    uint32_t codes = 0;
+    if (bad || d == 0.0f) {
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float u = __fmul_rn(__fsub_rn(x[j], m), rd);
-        float q = rintf(u);
-        if (fabsf(u - q) > 0.49999f) q = (float)rint(__ddiv_rn(__dsub_rn((double)x[j], (double)m), (double)d));
-        codes |= (uint32_t)(int)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * j);
+        for (int j = 0; j < 8; j++) x[j] = bad ? __int_as_float(0x7fffffff) : m;
+        return 0;
     }
+    const float rd = __frcp_rn(__fmul_rn(15.0f, d));
+    uint32_t codes = 0;
+    float q[8], far[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) { // (an integer's nearest: the low bits of 1.5 x 2^23 + 15 v)
+        const float v = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)), t = __fmaf_rn(v, 15.0f, 12582912.0f);
+        q[j] = __fsub_rn(t, 12582912.0f);
+        far[j] = fabsf(__fmaf_rn(v, 15.0f, -q[j]));
+        codes += __float_as_uint(t) * (1u << (4 * j));
+    }
+    codes -= 0x3f400000u; // (the sum of the constants that went in with the codes)
+    if (fmaxf(trx_a4_max3(trx_a4_max3(far[0], far[1], far[2]), far[3], far[4]), trx_a4_max3(far[5], far[6], far[7])) > 0.49998f) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (far[j] > 0.49998f) {
+                const float u = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)) * 15.0f, k = floorf(u);
+                const float h = __fmul_rn(__fadd_rn(k, 0.5f), d), s = __fadd_rn(m, h);
+                const float t = __fsub_rn(s, m); // s + lost = m + h
+                const float lost = __fadd_rn(__fsub_rn(m, __fsub_rn(s, t)), __fsub_rn(h, t));
+                const bool up = x[j] > s || (x[j] == s && (lost < 0.0f || (lost == 0.0f && ((int)k & 1))));
+                q[j] = up ? k + 1.0f : k;
+                codes = (codes & ~(15u << (4 * j))) | (uint32_t)(int)q[j] << (4 * j);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = __fmaf_rn(d, q[j], m); // (d x code is exact)
     return codes;
 }
 
-// where lane a (dims 8 a .. 8 a + 7) of a row at position p of a record finds its codes, scale and minimum
+// where lane a (dims 8 a .. 8 a + 7) of a row at position p of a record finds its codes, scale and minimum (p up to 63:
+// the block's second record)
 template <int HD> __device__ __forceinline__ int trx_a4_kcode(int p, int a) {
-    return p * (HD / 2) + ((a & 3) * TrxA4L<HD>::NG + (a >> 2)) * 4;
+    return (p >> 5) * TrxA4L<HD>::REC + (p & 31) * (HD / 2) + ((a & 3) * TrxA4L<HD>::NG + (a >> 2)) * 4;
 }
 template <int HD> __device__ __forceinline__ int trx_a4_vcode(int p, int a, int half) { // dims 8 a + 4 half ..
     constexpr int NG = TrxA4L<HD>::NG;
-    return TrxA4L<HD>::V + (p >> 3) * (4 * HD) + ((2 * (a & 3) + half) * 4 + ((p & 7) >> 1)) * (NG * 4) +
-           (a >> 2) * 4 + (p & 1) * 2;
+    return (p >> 5) * TrxA4L<HD>::REC + TrxA4L<HD>::V + ((p & 31) >> 3) * (4 * HD) +
+           ((2 * (a & 3) + half) * 4 + ((p & 7) >> 1)) * (NG * 4) + (a >> 2) * 4 + (p & 1) * 2;
 }
 template <int HD> __device__ __forceinline__ int trx_a4_pair(int p, int g) { // in a [pos / 2][g][pos % 2] plane
-    return (p >> 1) * (TrxA4L<HD>::NG * 4) + g * 4 + (p & 1) * 2;
+    return (p >> 5) * TrxA4L<HD>::REC + ((p & 31) >> 1) * (TrxA4L<HD>::NG * 4) + g * 4 + (p & 1) * 2;
 }
-template <int HD> __device__ __forceinline__ int trx_a4_km(int p, int g) {
-    return TrxA4L<HD>::KM + p * (TrxA4L<HD>::NG * 2) + g * 2;
+template <int HD> __device__ __forceinline__ int trx_a4_flat(int p, int g) { // in a [pos][g] plane
+    return (p >> 5) * TrxA4L<HD>::REC + (p & 31) * (TrxA4L<HD>::NG * 2) + g * 2;
 }
 
 // 8 values (dims 8 a ..) of a key / value row
 template <int HD> __device__ __forceinline__ void trx_a4_key8(const uint8_t *rec, int p, int a, float (&x)[8]) {
     const uint32_t w = *reinterpret_cast<const uint32_t *>(rec + trx_a4_kcode<HD>(p, a));
-    const float d = trx_half(*reinterpret_cast<const uint16_t *>(rec + TrxA4L<HD>::KD + trx_a4_pair<HD>(p, a >> 2)));
-    const float m = trx_half(*reinterpret_cast<const uint16_t *>(rec + trx_a4_km<HD>(p, a >> 2)));
+    const float d = trx_half(*reinterpret_cast<const uint16_t *>(rec + TrxA4L<HD>::KD + trx_a4_flat<HD>(p, a >> 2)));
+    const float m = trx_half(*reinterpret_cast<const uint16_t *>(rec + TrxA4L<HD>::KM + trx_a4_flat<HD>(p, a >> 2)));
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = __fmaf_rn(d, (float)((w >> (4 * j)) & 15), m); // (d x code is exact)
 }
@@ -186,78 +237,126 @@ template <int HD> __device__ __forceinline__ void trx_a4_value8(const uint8_t *r
 }
 
 // Writes an entry's rows of one block (blockIdx.x blocks after the entry's first) and KV head (blockIdx.y), HD / 8
-// lanes a row; then the block's bounds over all its 64 rows, which those rows may have changed: the lowest and highest
-// key value of each dim as 8-bit multiples (floor, ceil, at most 127) of the block's unit, the power of two that puts
-// their largest magnitude in [64, 128). A block with a NaN among its keys has the unit infinity. The rows that were
-// never written count too; such a block is no earlier one of any query, so that its bounds are not read.
+// lanes a row; and the block's bounds over all its 64 rows, which those rows may change: the lowest and highest key value
+// of each dim as 8-bit multiples (floor, ceil, at most 127) of the block's unit, the power of two that puts their largest
+// magnitude in [64, 128). A block with a NaN among its keys has the unit infinity. The rows that were never written
+// count too; such a block is no earlier one of any query, so that its bounds are not read.
+// The records are put together in shared memory (a row's value codes lie 2 bytes here and there) and leave it 16 bytes a
+// thread where the block is written whole, else as the rows' own pieces.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) trx_a4_write(TrxA4 a, TrxA4Batch b, const T *__restrict__ k, int64_t k_stride,
+__global__ void __launch_bounds__(256, 3) trx_a4_write(TrxA4 a, TrxA4Batch b, const T *__restrict__ k, int64_t k_stride,
                                                     const T *__restrict__ v, int64_t v_stride) {
-    constexpr int L = HD / 8, ROWS = 256 / L; // lanes a row, rows in flight
-    __shared__ float s_lo[ROWS][HD], s_hi[ROWS][HD];
-    __shared__ float s_max[HD / 32 + 1];
+    constexpr int L = HD / 8, ROWS = 256 / L, N = TRX_A4_BLOCK / ROWS; // lanes a row, rows in flight, passes
+    using Y = TrxA4L<HD>;
+    __shared__ __align__(16) uint8_t s_rec[Y::BLOCK];
+    __shared__ float s_lo[8][HD], s_hi[8][HD];
+    __shared__ float s_max[HD / 32];
     int slot, row0, rows, pos0;
     const int tid = threadIdx.x, kv = blockIdx.y, e = blockIdx.z;
     if (!trx_a4_entry(a, b, e, slot, row0, rows, pos0)) return;
     const int blk = pos0 / TRX_A4_BLOCK + blockIdx.x, first = blk * TRX_A4_BLOCK;
     if (first >= pos0 + rows) return;
+    const int64_t at = ((int64_t)slot * a.n_kv + kv) * a.n_blocks + blk;
+    uint8_t *rec = a.cache + at * Y::BLOCK;
+    const int p0 = max(pos0, first) - first, p1 = min(pos0 + rows - first, TRX_A4_BLOCK);
+    const int l = tid % L, g = l >> 2;
     int same = 0;
     for (int j = tid; j < e; j += 256) same |= b.slot[j] == slot;
+    float lo[8], hi[8];
+    int bad = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
     if (__syncthreads_or(same)) {
         if (tid == 0) atomicCAS(a.err, 0, TRX_A4_SAME_SLOT);
         return;
     }
-    const int64_t at = ((int64_t)slot * a.n_kv + kv) * a.n_blocks + blk;
-    uint8_t *rec = a.cache + at * TrxA4L<HD>::REC;
-    const int p0 = max(pos0, first) - first, p1 = min(pos0 + rows - first, TRX_A4_BLOCK);
-    const int l = tid % L, g = l >> 2;
-    for (int base = p0; base < p1; base += ROWS) {
-        const int p = base + tid / L;
-        const bool on = p < p1;
-        const int64_t row = row0 + (first + (on ? p : p0) - pos0);
-        float x[8];
+#pragma unroll 1
+    for (int i = 0; i < N; i += 2) { // two rows a lane
+        int p[2];
+        bool on[2];
+        TrxA4Raw<T> rk[2], rv[2];
+        float x[2][8];
         uint16_t d, m;
-        trx_a4_load8(k + row * k_stride + kv * HD + 8 * l, x);
-        uint32_t c = trx_a4_quant(x, d, m);
-        if (on) {
-            *reinterpret_cast<uint32_t *>(rec + trx_a4_kcode<HD>(p, l)) = c;
-            if ((l & 3) == 0) {
-                *reinterpret_cast<uint16_t *>(rec + TrxA4L<HD>::KD + trx_a4_pair<HD>(p, g)) = d;
-                *reinterpret_cast<uint16_t *>(rec + trx_a4_km<HD>(p, g)) = m;
-            }
-        }
-        trx_a4_load8(v + row * v_stride + kv * HD + 8 * l, x);
-        c = trx_a4_quant(x, d, m);
-        if (on) {
-            *reinterpret_cast<uint16_t *>(rec + trx_a4_vcode<HD>(p, l, 0)) = (uint16_t)c;
-            *reinterpret_cast<uint16_t *>(rec + trx_a4_vcode<HD>(p, l, 1)) = (uint16_t)(c >> 16);
-            if ((l & 3) == 0) {
-                *reinterpret_cast<uint16_t *>(rec + TrxA4L<HD>::VD + trx_a4_pair<HD>(p, g)) = d;
-                *reinterpret_cast<uint16_t *>(rec + TrxA4L<HD>::VM + trx_a4_pair<HD>(p, g)) = m;
-            }
-        }
-    }
-    __syncthreads();
-    float lo[8], hi[8], x[8];
-    int bad = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
-    for (int p = tid / L; p < TRX_A4_BLOCK; p += ROWS) {
-        trx_a4_key8<HD>(rec, p, l, x);
+        for (int r = 0; r < 2; r++) {
+            p[r] = (i + r) * ROWS + tid / L;
+            on[r] = p[r] >= p0 && p[r] < p1;
+            const int64_t row = row0 + (int64_t)(first + p[r] - pos0);
+            if (on[r]) {
+                rk[r] = trx_a4_raw8(k + row * k_stride + kv * HD + 8 * l);
+                rv[r] = trx_a4_raw8(v + row * v_stride + kv * HD + 8 * l);
+            } else rk[r] = rv[r] = TrxA4Raw<T>{};
+        }
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            trx_a4_floats(rk[r], x[r]);
+            if (__any_sync(0xffffffffu, on[r])) {
+                const uint32_t c = trx_a4_quant(x[r], d, m);
+                if (on[r]) {
+                    *reinterpret_cast<uint32_t *>(s_rec + trx_a4_kcode<HD>(p[r], l)) = c;
+                    if ((l & 3) == 0) {
+                        *reinterpret_cast<uint16_t *>(s_rec + Y::KD + trx_a4_flat<HD>(p[r], g)) = d;
+                        *reinterpret_cast<uint16_t *>(s_rec + Y::KM + trx_a4_flat<HD>(p[r], g)) = m;
+                    }
+                }
+            }
+            if (!on[r]) trx_a4_key8<HD>(rec, p[r], l, x[r]); // a row that stays
+            bad |= x[r][0] != x[r][0];                       // (a group's values are NaN together)
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) lo[j] = trx_a4_min3(lo[j], x[0][j], x[1][j]), hi[j] = trx_a4_max3(hi[j], x[0][j], x[1][j]);
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+            if (__any_sync(0xffffffffu, on[r])) {
+                trx_a4_floats(rv[r], x[r]);
+                const uint32_t c = trx_a4_quant(x[r], d, m);
+                if (on[r]) {
+                    *reinterpret_cast<uint16_t *>(s_rec + trx_a4_vcode<HD>(p[r], l, 0)) = (uint16_t)c;
+                    *reinterpret_cast<uint16_t *>(s_rec + trx_a4_vcode<HD>(p[r], l, 1)) = (uint16_t)(c >> 16);
+                    if ((l & 3) == 0) {
+                        *reinterpret_cast<uint16_t *>(s_rec + Y::VD + trx_a4_pair<HD>(p[r], g)) = d;
+                        *reinterpret_cast<uint16_t *>(s_rec + Y::VM + trx_a4_pair<HD>(p[r], g)) = m;
+                    }
+                }
+            }
+    }
+    // the lanes that share dims in a warp, then the warps
+#pragma unroll
+    for (int s = L; s < 32; s <<= 1)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            lo[j] = fminf(lo[j], x[j]);
-            hi[j] = fmaxf(hi[j], x[j]);
-            bad |= x[j] != x[j];
+            lo[j] = fminf(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], s));
+            hi[j] = fmaxf(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], s));
+        }
+    if ((tid & 31) < L) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) s_lo[tid >> 5][8 * l + j] = lo[j], s_hi[tid >> 5][8 * l + j] = hi[j];
+    }
+    bad = __syncthreads_or(bad);
+    if (p0 == 0 && p1 == TRX_A4_BLOCK) {
+        for (int i = tid; i < Y::BLOCK / 16; i += 256) reinterpret_cast<uint4 *>(rec)[i] = reinterpret_cast<const uint4 *>(s_rec)[i];
+    } else {
+        for (int p = p0 + tid / L; p < p1; p += ROWS) {
+            auto copy = [&](int off, auto t) {
+                using U = decltype(t);
+                *reinterpret_cast<U *>(rec + off) = *reinterpret_cast<const U *>(s_rec + off);
+            };
+            copy(trx_a4_kcode<HD>(p, l), uint32_t());
+            copy(trx_a4_vcode<HD>(p, l, 0), uint16_t());
+            copy(trx_a4_vcode<HD>(p, l, 1), uint16_t());
+            if ((l & 3) == 0) {
+                copy(Y::KD + trx_a4_flat<HD>(p, g), uint16_t());
+                copy(Y::KM + trx_a4_flat<HD>(p, g), uint16_t());
+                copy(Y::VD + trx_a4_pair<HD>(p, g), uint16_t());
+                copy(Y::VM + trx_a4_pair<HD>(p, g), uint16_t());
+            }
         }
     }
-#pragma unroll
-    for (int j = 0; j < 8; j++) s_lo[tid / L][8 * l + j] = lo[j], s_hi[tid / L][8 * l + j] = hi[j];
-    bad = __syncthreads_or(bad);
     float l1 = 0.0f, h1 = 0.0f;
     if (tid < HD) {
         l1 = s_lo[0][tid], h1 = s_hi[0][tid];
-        for (int r = 1; r < ROWS; r++) l1 = fminf(l1, s_lo[r][tid]), h1 = fmaxf(h1, s_hi[r][tid]);
+#pragma unroll
+        for (int r = 1; r < 8; r++) l1 = fminf(l1, s_lo[r][tid]), h1 = fmaxf(h1, s_hi[r][tid]);
         float most = fmaxf(fabsf(l1), fabsf(h1));
         for (int s = 16; s; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
         if ((tid & 31) == 0) s_max[tid >> 5] = most;
@@ -270,113 +369,640 @@ __global__ void __launch_bounds__(256) trx_a4_write(TrxA4 a, TrxA4Batch b, const
         if (most > 0.0f && !bad) frexpf(most, &ex);
         // (keys are multiples of 2^-24 up to 65504 x 16: the unit is a normal float)
         const float unit = __int_as_float((ex - 7 + 127) << 23), per = __int_as_float((7 - ex + 127) << 23);
-        int8_t *o = a.bounds + at * (2 * HD) + (tid >> 3) * 16 + (tid & 7);
+        int8_t *o = a.bounds + at * (2 * HD) + tid;
         o[0] = bad ? 0 : (int8_t)fmaxf(floorf(__fmul_rn(l1, per)), -127.0f);
-        o[8] = bad ? 0 : (int8_t)fminf(ceilf(__fmul_rn(h1, per)), 127.0f);
+        o[HD] = bad ? 0 : (int8_t)fminf(ceilf(__fmul_rn(h1, per)), 127.0f);
         if (tid == 0) a.units[at] = bad ? INFINITY : unit;
     }
 }
 
-// The rows of an entry's block read back (the write's grid)
+// The rows of an entry's block read back (the write's grid), by way of shared memory
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__restrict__ k, int64_t k_stride,
                                                    T *__restrict__ v, int64_t v_stride) {
     constexpr int L = HD / 8, ROWS = 256 / L;
+    __shared__ __align__(16) uint8_t s_rec[TrxA4L<HD>::BLOCK];
     int slot, row0, rows, pos0;
     const int tid = threadIdx.x, kv = blockIdx.y;
     if (!trx_a4_entry(a, b, blockIdx.z, slot, row0, rows, pos0)) return;
     const int blk = pos0 / TRX_A4_BLOCK + blockIdx.x, first = blk * TRX_A4_BLOCK;
-    const uint8_t *rec = a.cache + (((int64_t)slot * a.n_kv + kv) * a.n_blocks + blk) * TrxA4L<HD>::REC;
+    if (first >= pos0 + rows) return;
+    const uint8_t *rec = a.cache + (((int64_t)slot * a.n_kv + kv) * a.n_blocks + blk) * TrxA4L<HD>::BLOCK;
+    for (int i = tid; i < TrxA4L<HD>::BLOCK / 16; i += 256)
+        reinterpret_cast<uint4 *>(s_rec)[i] = reinterpret_cast<const uint4 *>(rec)[i];
+    __syncthreads();
     const int p0 = max(pos0, first) - first, p1 = min(pos0 + rows - first, TRX_A4_BLOCK), l = tid % L;
     for (int p = p0 + tid / L; p < p1; p += ROWS) {
         const int64_t row = row0 + (first + p - pos0);
         float x[8];
-        trx_a4_key8<HD>(rec, p, l, x);
+        trx_a4_key8<HD>(s_rec, p, l, x);
         trx_a4_store8(k + row * k_stride + kv * HD + 8 * l, x);
-        trx_a4_value8<HD>(rec, p, l, x);
+        trx_a4_value8<HD>(s_rec, p, l, x);
         trx_a4_store8(v + row * v_stride + kv * HD + 8 * l, x);
     }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Attention: the simple form. A CTA a (query row, KV head); a head of the group after another: 8 warps take a listed
-// block each in turn, lane l the dims 8 (l % (HD / 8)) of every second (fourth) position, with a running maximum and
-// sum; the warps' results are joined through shared memory.
-// list: the blocks to attend to (select), or NULL: blocks 0 .. n_list - 1.
-template <int HD, typename T>
-__device__ void trx_a4_attend_row(const TrxA4 &a, const uint8_t *recs, const int *list, int n_list, int pos,
-                                  const T *q, float scale, T *out) {
-    constexpr int L = HD / 8, PER = 32 / L, W = 8;
-    __shared__ float s_m[W], s_l[W], s_o[W][HD];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = lane % L;
-    float qx[8], o[8], x[8], m = -INFINITY, sum = 0.0f;
-    trx_a4_load8(q + 8 * l, qx);
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = 0.0f;
-    for (int i = warp; i < n_list; i += W) {
-        const int blk = list ? list[i] : i;
-        const uint8_t *rec = recs + (int64_t)blk * TrxA4L<HD>::REC;
-        for (int p0 = 0; p0 < TRX_A4_BLOCK && blk * TRX_A4_BLOCK + p0 <= pos; p0 += PER) {
-            const int p = p0 + lane / L;
-            trx_a4_key8<HD>(rec, p, l, x);
-            float s = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; j++) s = __fmaf_rn(qx[j], x[j], s);
-            for (int w = 1; w < L; w <<= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-            s *= scale;
-            if (blk * TRX_A4_BLOCK + p > pos) continue; // (only lanes leave: the shuffles above are done)
-            const float mn = fmaxf(m, s);
-            // a NaN score makes the row NaN; -inf beside -inf adds nothing
-            const float f = m == mn ? 1.0f : expf(m - mn), w = s == -INFINITY ? 0.0f : expf(s - mn);
-            trx_a4_value8<HD>(rec, p, l, x);
-            m = s != s ? s : mn;
-            sum = __fmaf_rn(sum, f, w);
-#pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = __fmaf_rn(w, x[j], o[j] * f);
-        }
-        __syncwarp();
-    }
-    (void)a;
-    for (int w = L; w < 32; w <<= 1) { // the positions that lanes took side by side
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, w), sum2 = __shfl_xor_sync(0xffffffffu, sum, w);
-        const float mn = fmaxf(m, m2), f = m == mn ? 1.0f : expf(m - mn), f2 = m2 == mn ? 1.0f : expf(m2 - mn);
-        sum = sum * f + sum2 * f2;
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = o[j] * f + __shfl_xor_sync(0xffffffffu, o[j], w) * f2;
-        m = mn;
-    }
-    __syncthreads(); // (the head before has been read)
-    if (lane < L) {
-        if (lane == 0) s_m[warp] = m, s_l[warp] = sum;
-        for (int j = 0; j < 8; j++) s_o[warp][8 * l + j] = o[j];
-    }
-    __syncthreads();
-    if (tid < L) {
-        float M = -INFINITY, S = 0.0f;
-        for (int w = 0; w < W; w++) M = fmaxf(M, s_m[w]);
-        for (int j = 0; j < 8; j++) o[j] = 0.0f;
-        for (int w = 0; w < W; w++) {
-            const float f = s_m[w] == M ? 1.0f : expf(s_m[w] - M);
-            S += s_l[w] * f;
-            for (int j = 0; j < 8; j++) o[j] += s_o[w][8 * tid + j] * f;
-        }
-        for (int j = 0; j < 8; j++) o[j] = S == 0.0f ? 0.0f : __fdiv_rn(o[j], S);
-        trx_a4_store8(out + 8 * tid, o);
+// Attention.
+//
+// With the query x = q 2^-e of a row, a key's score is scale 2^e sum_g (d_g sum_i x_gi c_gi + m_g sum_i x_gi), and an
+// output group is (sum_t (p_t d_tg) c_tg + sum_t p_t m_tg) / sum_t p_t: the codes go into the tensor cores as they
+// are, and scales and minima are applied to a 32nd of the values.
+//
+// Codes as f16: four bits masked out of a word (c or 16 c in each half) are an f16 subnormal, c 2^-24 or 16 c 2^-24,
+// exactly: a word of 8 codes is one shift and four ANDs, and no subtraction of a bias. The query values that meet a
+// 16 c are stored divided by 16; the outputs that come of one are divided by 16 at the end, where 2^24 goes too.
+//
+// A warp takes records of 32 positions through its own ring of two bulk copies, 16 positions at a time:
+//   scores   mma m16n8k16: A = 16 keys x 16 codes, B = 8 query rows (f32 rows: a second B with what f16 drops of the
+//            first); a group is two of them, then d; the minima's sums are one m16n8k8 with B = sum_i x_gi in two f16
+//            parts
+//   softmax  running maximum a row; p in f16 (f32 rows: two f16 parts, 22 bits), transposed in registers (movmatrix)
+//   outputs  mma m16n8k16: A = 16 dims x 16 positions of codes, B = p_t d_tg of 8 rows; one more with the minima (and
+//            ones, which sum p) as A.
+// 16 query rows of f16 or bf16 type, or 8 (R), share the codes' unpacking; scores, sums and outputs are f32.
+// p stays below 2^15 / max(1, d): the reference that is subtracted in the exponent is the row's maximum so far, plus
+// the binary logarithm of the largest value scale so far where it is above 1, less a constant.
+//
+// A cluster of CTAs shares one tile of query rows: its warps take records in turn, their results are joined in each
+// CTA through shared memory, and the CTAs' through distributed shared memory, so that no workspace or second launch is
+// needed and overlapping calls share nothing.
+#define TRX_A4_WARPS 8
+#define TRX_A4_STAGES 2
+
+__device__ __forceinline__ void trx_a4_mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void trx_a4_mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(b0));
+}
+// an 8 x 8 matrix of f16 pairs (lane: row l / 4, columns 2 (l % 4), + 1), transposed
+__device__ __forceinline__ uint32_t trx_a4_transpose(uint32_t a) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ trx_f2 trx_fma2(trx_f2 a, trx_f2 b, trx_f2 c) {
+    trx_f2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+// 2^x within 2^-22 (relative), 0 for -inf
+__device__ __forceinline__ float trx_a4_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t trx_a4_half2(float lo, float hi) { return trx_a4_pack2(lo, hi, (const __half *)nullptr); }
+__device__ __forceinline__ float2 trx_a4_float2(uint32_t h) { return __half22float2(*reinterpret_cast<const __half2 *>(&h)); }
+__device__ __forceinline__ uint32_t trx_a4_hmul2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t trx_a4_hadd2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t trx_a4_hfma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+// NW consecutive words of shared memory
+template <int NW> __device__ __forceinline__ void trx_a4_lds(const uint8_t *p, uint32_t (&w)[NW]) {
+    if constexpr (NW == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (NW == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else w[0] = *reinterpret_cast<const uint32_t *>(p);
+}
+
+__device__ __forceinline__ uint32_t trx_a4_cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void trx_a4_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// the address of CTA rank's copy of a shared variable, in the cluster's window
+__device__ __forceinline__ uint32_t trx_a4_peer(const void *p, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(trx_smem(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float4 trx_a4_peer_load4(uint32_t a) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ float trx_a4_peer_load(uint32_t a) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a));
+    return v;
+}
+
+template <int HD, int R> struct TrxA4Tile { // shared memory of a tile of R query rows
+    static constexpr int W = TRX_A4_WARPS, RING = W * TRX_A4_STAGES * TrxA4L<HD>::REC, PARTS = W * R * (HD + 2) * 4;
+    static constexpr int PART = RING > PARTS ? RING : PARTS; // the ring, then in its place the warps' results
+    static constexpr int SMEM = PART + R * (HD + 2) * 4;     // behind them the CTA's result
+};
+
+// A call's query and output rows: rows of type f32 (F32), else bf16 or f16
+struct TrxA4Rows {
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    int bf16;
+};
+template <bool F32> __device__ __forceinline__ void trx_a4_q8(const TrxA4Rows &io, int64_t at, float (&x)[8]) {
+    if constexpr (F32) trx_a4_load8((const float *)io.q + at, x);
+    else if (io.bf16) trx_a4_load8((const __nv_bfloat16 *)io.q + at, x);
+    else trx_a4_load8((const __half *)io.q + at, x);
+}
+template <bool F32> __device__ __forceinline__ float trx_a4_q1(const TrxA4Rows &io, int64_t at) {
+    if constexpr (F32) return ((const float *)io.q)[at];
+    const uint16_t u = ((const uint16_t *)io.q)[at];
+    return io.bf16 ? trx_bf16(u) : trx_half(u);
+}
+template <bool F32> __device__ __forceinline__ void trx_a4_out4(const TrxA4Rows &io, int64_t at, float4 v) {
+    if constexpr (F32) *reinterpret_cast<float4 *>((float *)io.out + at) = v;
+    else if (io.bf16)
+        *reinterpret_cast<uint2 *>((__nv_bfloat16 *)io.out + at) =
+            make_uint2(trx_a4_pack2(v.x, v.y, (const __nv_bfloat16 *)nullptr), trx_a4_pack2(v.z, v.w, (const __nv_bfloat16 *)nullptr));
+    else
+        *reinterpret_cast<uint2 *>((__half *)io.out + at) = make_uint2(trx_a4_half2(v.x, v.y), trx_a4_half2(v.z, v.w));
+}
+
+// The 8 codes of a word as four pairs of f16, in the order of bits 0, 4, 8, 12 of its halves: the integers themselves
+// (EXACT), or c 2^-24, 16 c 2^-24, c 2^-24, 16 c 2^-24
+template <bool EXACT> __device__ __forceinline__ void trx_a4_codes(uint32_t w, uint32_t (&h)[4]) {
+    const uint32_t v = w >> 8;
+    if constexpr (EXACT) { // 1024 + c and 1024 + 16 c from their bits
+        h[0] = trx_a4_hadd2((w & 0x000f000fu) | 0x64006400u, 0xe400e400u);
+        h[1] = trx_a4_hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u);
+        h[2] = trx_a4_hadd2((v & 0x000f000fu) | 0x64006400u, 0xe400e400u);
+        h[3] = trx_a4_hfma2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u);
+    } else {
+        h[0] = w & 0x000f000fu, h[1] = w & 0x00f000f0u, h[2] = v & 0x000f000fu, h[3] = v & 0x00f000f0u;
     }
 }
 
-template <int HD, typename T>
-__global__ void __launch_bounds__(256) trx_a4_attend(TrxA4 a, TrxA4Batch b, const T *__restrict__ q, int64_t q_stride,
-                                                     float scale, T *__restrict__ out, int64_t out_stride) {
+// One warp's state for R query rows: NT tiles of 8
+template <int HD, bool F32, int R> struct TrxA4Warp {
+    static constexpr bool EXACT = F32;
+    static constexpr int NG = HD / 32, NT = R / 8, NB = F32 ? 2 : NT;
+    static_assert(R == 8 || (R == 16 && !F32), "8 rows, or 16 of a 16-bit type");
+    // scores of 16-bit types may pass the reference by 2^LAZY before the sums are rescaled
+    static constexpr float LAZY = F32 ? 0.0f : 8.0f, TOP = F32 ? 14.0f : 7.0f;
+    uint32_t qb[NB][2 * NG][2]; // the query fragments: lane (n = lane / 4, c = lane % 4) has row n (+ 8)
+    uint32_t qs[NT];            // their groups' sums
+    int lim[NT];                // the last position row n (+ 8) sees; -1: no row
+    float c[NT][2];             // rows 2 c, 2 c + 1 (+ 8): the scores' factor, with log2(e),
+    float top[NT][2], ref[NT][2]; // the running maximum, and what the exponent subtracts
+    float ed, edlim;            // binary logarithm of the largest value scale so far, at least 0, and its power
+    float acc[NG][2][NT][4], accm[NT][4];
+
+    // the query rows of the tile: row r of it is at off(r); rows past n_rows are zero
+    template <typename Off>
+    __device__ __forceinline__ void load(const TrxA4Rows &io, int lane, int n_rows, float scale, Off off) {
+        const int n = lane >> 2, cc = lane & 3;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const bool on = n + 8 * t < n_rows;
+            const int64_t at = on ? off(n + 8 * t) : 0;
+            float x[NG][8], most = 0.0f, sum[NG];
+            bool bad = false;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[g][j] = 0.0f;
+                if (on) trx_a4_q8<F32>(io, at + 32 * g + 8 * cc, x[g]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    most = fmaxf(most, fabsf(x[g][j]));
+                    bad |= !(fabsf(x[g][j]) <= 3.402823466e38f);
+                }
+            }
+#pragma unroll
+            for (int s = 1; s <= 2; s <<= 1) {
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
+                bad |= __shfl_xor_sync(0xffffffffu, (int)bad, s) != 0;
+            }
+            // x = q 2^(10 - ex), below 2^10: a group's sum is below 2^15
+            int ex = 0;
+            if (!bad && most > 0.0f) ex = max((int)((__float_as_uint(most) >> 23) & 255) - 126, -100);
+            const float f = __int_as_float((10 - ex + 127) << 23) * (scale < 0.0f ? -1.0f : 1.0f);
+            // (2^24: the codes are subnormals; capped, so that a score of 0 stays 0)
+            float factor = fminf(fabsf(scale) * 1.44269504088896341f *
+                                     __int_as_float((min(ex, 113) + (EXACT ? -10 : 14) + 127) << 23), 3.0e38f);
+            if (bad) factor = __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                c[t][i] = __shfl_sync(0xffffffffu, factor, 4 * (2 * cc + i));
+                top[t][i] = ref[t][i] = -1.0e30f;
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                sum[g] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    x[g][j] = bad ? 0.0f : x[g][j] * f;
+                    sum[g] += x[g][j];
+                    if (!EXACT && (j & 1)) x[g][j] *= 0.0625f;
+                }
+#pragma unroll
+                for (int s = 1; s <= 2; s <<= 1) sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], s);
+                // (fragment register, its two dims): (0: 0, 4) (1: 1, 5) of the first k16, (0: 2, 6) (1: 3, 7) of the second
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int o = 0; o < 2; o++) {
+                        const float lo = x[g][2 * h + o], hi = x[g][2 * h + o + 4];
+                        const uint32_t w = trx_a4_half2(lo, hi);
+                        qb[F32 ? 0 : t][2 * g + h][o] = w;
+                        if constexpr (F32) {
+                            const float2 b = trx_a4_float2(w);
+                            qb[1][2 * g + h][o] = trx_a4_half2(lo - b.x, hi - b.y);
+                        }
+                    }
+            }
+            uint32_t w[4];
+#pragma unroll
+            for (int g = 0; g < NG; g += 2) {
+                w[g / 2] = trx_a4_half2(sum[g], sum[g + 1]);
+                const float2 b = trx_a4_float2(w[g / 2]);
+                w[NG / 2 + g / 2] = trx_a4_half2(sum[g] - b.x, sum[g + 1] - b.y);
+            }
+            if constexpr (NG == 4) qs[t] = cc == 0 ? w[0] : cc == 1 ? w[1] : cc == 2 ? w[2] : w[3];
+            else qs[t] = cc == 0 ? w[0] : cc == 1 ? w[1] : 0u;
+#pragma unroll
+            for (int i = 0; i < 4; i++) accm[t][i] = 0.0f;
+#pragma unroll
+            for (int g = 0; g < NG; g++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[g][h][t][i] = 0.0f;
+        }
+        ed = 0.0f, edlim = 1.0f;
+    }
+
+    // one record (32 positions from pos0); MASK: some row does not see all of them
+    template <bool MASK> __device__ __forceinline__ void record(const uint8_t *rec, int lane, int pos0) {
+        using L = TrxA4L<HD>;
+        const int n = lane >> 2, cc = lane & 3;
+        float s[2][NT][4]; // 16 positions each: n (0, 1) and n + 8 (2, 3) x rows 2 cc, 2 cc + 1
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint8_t *p0 = rec + (16 * t + n) * (HD / 2) + cc * (NG * 4);
+            const uint8_t *ps = rec + L::KD + (16 * t + n) * (NG * 2);
+            uint32_t w0[NG], w1[NG], d0[NG / 2], d1[NG / 2], m[2];
+            trx_a4_lds<NG>(p0, w0);
+            trx_a4_lds<NG>(p0 + 8 * (HD / 2), w1);
+            trx_a4_lds<NG / 2>(ps, d0);
+            trx_a4_lds<NG / 2>(ps + 8 * (NG * 2), d1);
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                m[k] = *reinterpret_cast<const uint32_t *>(ps + (L::KM - L::KD) + 8 * k * (NG * 2) + (NG == 4 ? (cc & 1) * 4 : 0));
+            trx_f2 a[NT][2];
+#pragma unroll
+            for (int r = 0; r < NT; r++) {
+                float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                trx_a4_mma8(e, m[0], m[1], qs[r]);
+                a[r][0] = trx_pack2(e[0], e[1]), a[r][1] = trx_pack2(e[2], e[3]);
+                if constexpr (!EXACT) {
+                    const trx_f2 tiny = trx_pack2(5.9604644775390625e-8f, 5.9604644775390625e-8f); // 2^-24
+                    a[r][0] = trx_mul2(a[r][0], tiny), a[r][1] = trx_mul2(a[r][1], tiny);
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                uint32_t u[4], v[4];
+                trx_a4_codes<EXACT>(w0[g], u);
+                trx_a4_codes<EXACT>(w1[g], v);
+                const float2 e0 = trx_a4_float2(d0[g / 2]), e1 = trx_a4_float2(d1[g / 2]);
+                const float f0 = g & 1 ? e0.y : e0.x, f1 = g & 1 ? e1.y : e1.x;
+#pragma unroll
+                for (int r = 0; r < NT; r++) {
+                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int b = r; b < NB; b += NT) {
+                        trx_a4_mma16(x, u[0], v[0], u[1], v[1], qb[b][2 * g][0], qb[b][2 * g][1]);
+                        trx_a4_mma16(x, u[2], v[2], u[3], v[3], qb[b][2 * g + 1][0], qb[b][2 * g + 1][1]);
+                    }
+                    a[r][0] = trx_fma2(trx_pack2(x[0], x[1]), trx_pack2(f0, f0), a[r][0]);
+                    a[r][1] = trx_fma2(trx_pack2(x[2], x[3]), trx_pack2(f1, f1), a[r][1]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < NT; r++) {
+                s[t][r][0] = trx_lo(a[r][0]), s[t][r][1] = trx_hi(a[r][0]);
+                s[t][r][2] = trx_lo(a[r][1]), s[t][r][3] = trx_hi(a[r][1]);
+            }
+        }
+        // the largest value scale of the record, where it passes those before
+        bool grow = false;
+        {
+            uint32_t w[NG / 2];
+            trx_a4_lds<NG / 2>(rec + L::VD + lane * (NG * 2), w);
+            float2 f = trx_a4_float2(w[0]);
+            float big = fmaxf(f.x, f.y);
+            if constexpr (NG == 4) {
+                f = trx_a4_float2(w[NG / 2 - 1]);
+                big = fmaxf(big, fmaxf(f.x, f.y));
+            }
+            if (__any_sync(0xffffffffu, big > edlim)) {
+                for (int x = 16; x; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+                const int e = (int)((__float_as_uint(big) >> 23) & 255) - 126; // 2^e > big
+                ed = (float)e, edlim = __int_as_float((e + 127) << 23);
+                grow = true;
+            }
+        }
+        float f[NT][2];
+#pragma unroll
+        for (int r = 0; r < NT; r++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int last = MASK ? __shfl_sync(0xffffffffu, lim[r], 4 * (2 * cc + i)) : 0;
+                float best = -INFINITY;
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        float &x = s[t][r][2 * k + i];
+                        x *= c[r][i];
+                        if (MASK && pos0 + 16 * t + 8 * k + n > last) x = -INFINITY;
+                        best = fmaxf(best, x);
+                    }
+#pragma unroll
+                for (int x = 4; x <= 16; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
+                grow |= best > top[r][i] + LAZY;
+                f[r][i] = best;
+            }
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int r = 0; r < NT; r++) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    top[r][i] = fmaxf(top[r][i], f[r][i]);
+                    const float to = top[r][i] == -1.0e30f ? -1.0e30f : top[r][i] + ed - TOP;
+                    f[r][i] = ref[r][i] == to ? 1.0f : trx_a4_exp2(ref[r][i] - to);
+                    ref[r][i] = to;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) accm[r][i] *= f[r][i & 1];
+#pragma unroll
+                for (int g = 0; g < NG; g++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[g][h][r][i] *= f[r][i & 1];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; t++) { // 16 positions: two tiles of 8
+            uint32_t w[2][NG], d[2][NG], m[2], p[2][NT], pl[2], ok[2][NT];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                trx_a4_lds<NG>(rec + L::V + (2 * t + k) * (4 * HD) + lane * (NG * 4), w[k]);
+                trx_a4_lds<NG>(rec + L::VD + (8 * t + 4 * k + cc) * (NG * 4), d[k]);
+                // rows 0 .. NG - 1 of A are the groups' minima, row NG ones
+                m[k] = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VM + (8 * t + 4 * k + cc) * (NG * 4) + n * 4)
+                              : n == NG ? 0x3c003c00u : 0u;
+#pragma unroll
+                for (int r = 0; r < NT; r++) {
+                    const float x = trx_a4_exp2(s[t][r][2 * k] - ref[r][0]), y = trx_a4_exp2(s[t][r][2 * k + 1] - ref[r][1]);
+                    const uint32_t h = trx_a4_half2(x, y);
+                    p[k][r] = trx_a4_transpose(h);
+                    if constexpr (F32) {
+                        const float2 b = trx_a4_float2(h);
+                        pl[k] = trx_a4_transpose(trx_a4_half2(x - b.x, y - b.y));
+                    }
+                    // (a masked position's scale may be a NaN)
+                    if constexpr (MASK) {
+                        const int at = pos0 + 16 * t + 8 * k + 2 * cc;
+                        ok[k][r] = (at <= lim[r] ? 0xffffu : 0u) | (at + 1 <= lim[r] ? 0xffff0000u : 0u);
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < NT; r++) {
+                trx_a4_mma16(accm[r], m[0], 0u, m[1], 0u, p[0][r], p[1][r]);
+                if constexpr (F32) trx_a4_mma16(accm[r], m[0], 0u, m[1], 0u, pl[0], pl[1]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                uint32_t u[4], v[4];
+                trx_a4_codes<EXACT>(w[0][g], u);
+                trx_a4_codes<EXACT>(w[1][g], v);
+#pragma unroll
+                for (int r = 0; r < NT; r++) {
+                    uint32_t b0 = trx_a4_hmul2(p[0][r], d[0][g]), b1 = trx_a4_hmul2(p[1][r], d[1][g]);
+                    if constexpr (F32) { // p d in two parts: what the product's rounding drops, and the lower part's product
+                        uint32_t l0 = trx_a4_hfma2(pl[0], d[0][g], trx_a4_hfma2(p[0][r], d[0][g], b0 ^ 0x80008000u));
+                        uint32_t l1 = trx_a4_hfma2(pl[1], d[1][g], trx_a4_hfma2(p[1][r], d[1][g], b1 ^ 0x80008000u));
+                        if constexpr (MASK) l0 &= ok[0][r], l1 &= ok[1][r];
+                        trx_a4_mma16(acc[g][0][r], u[0], u[1], v[0], v[1], l0, l1);
+                        trx_a4_mma16(acc[g][1][r], u[2], u[3], v[2], v[3], l0, l1);
+                    }
+                    if constexpr (MASK) b0 &= ok[0][r], b1 &= ok[1][r];
+                    trx_a4_mma16(acc[g][0][r], u[0], u[1], v[0], v[1], b0, b1);
+                    trx_a4_mma16(acc[g][1][r], u[2], u[3], v[2], v[3], b0, b1);
+                }
+            }
+        }
+    }
+
+    // this warp's rows into o [R][HD] (not yet divided) with their references and sums
+    __device__ __forceinline__ void store(int lane, float *o, float *refs, float *sums) {
+        const int n = lane >> 2, cc = lane & 3;
+#pragma unroll
+        for (int r = 0; r < NT; r++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) { // query row 2 cc + i
+                const int row = 8 * r + 2 * cc + i;
+                if (n == 0) refs[row] = ref[r][i];
+                if (n == NG) sums[row] = accm[r][i];
+#pragma unroll
+                for (int g = 0; g < NG; g++) { // dims 32 g + 4 n + 0..3
+                    const float m = __shfl_sync(0xffffffffu, accm[r][i], 4 * g + cc);
+                    const float e = EXACT ? 1.0f : 16777216.0f, f = EXACT ? 1.0f : 1048576.0f; // 2^24, 2^20
+                    *reinterpret_cast<float4 *>(o + row * HD + 32 * g + 4 * n) =
+                        make_float4(__fmaf_rn(acc[g][0][r][i], e, m), __fmaf_rn(acc[g][0][r][2 + i], f, m),
+                                    __fmaf_rn(acc[g][1][r][i], e, m), __fmaf_rn(acc[g][1][r][2 + i], f, m));
+                }
+            }
+    }
+};
+
+// A tile of query rows (row r: its values at off_q(r) and off_o(r), its last position lim(r)) over the first n_units
+// records (of the listed blocks, or 0, 1, ..), by the CTAs of the cluster (ranks of them). smem: TrxA4Tile::SMEM bytes,
+// 128-byte aligned; no copy may be in flight into it, and what was read of it is ordered before (the caller's barrier).
+template <int HD, bool F32, int R, typename Lim, typename OffQ, typename OffO>
+__device__ __forceinline__ void trx_a4_tile(uint8_t *smem, int32_t *err, const TrxA4Rows &io, const uint8_t *recs,
+                                            const int *list, int n_units, int n_rows, int last, float scale, int ranks,
+                                            Lim lim, OffQ off_q, OffO off_o) {
+    constexpr int REC = TrxA4L<HD>::REC, S = TRX_A4_STAGES, W = TRX_A4_WARPS;
+    __shared__ __align__(8) uint64_t full[W][S];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = ranks > 1 ? (int)trx_a4_cluster_rank() : 0;
+    // (a warp uses its own barriers only)
+    if (lane == 0) {
+        for (int i = 0; i < S; i++) trx_mbar_init(&full[warp][i], 1);
+        trx_fence_barrier_init();
+    }
+    __syncwarp();
+    uint8_t *ring = smem + warp * (S * REC);
+    const int step = ranks * W;
+    auto record = [&](int u) { return list ? 2 * list[u >> 1] + (u & 1) : u; }; // the u-th record's index
+    auto fetch = [&](int u, int st) {
+        trx_mbar_expect_tx(&full[warp][st], REC);
+        trx_bulk_g2s(ring + st * REC, recs + (int64_t)record(u) * REC, REC, &full[warp][st]);
+    };
+    int u = rank * W + warp;
+    if (lane == 0)
+        for (int i = 0; i < S; i++)
+            if (u + i * step < n_units) fetch(u + i * step, i);
+    TrxA4Warp<HD, F32, R> w;
+    w.load(io, lane, n_rows, scale, off_q);
+    int low = last; // the lowest of the rows' last positions
+#pragma unroll
+    for (int t = 0; t < R / 8; t++) {
+        const int r = (lane >> 2) + 8 * t;
+        w.lim[t] = r < n_rows ? lim(r) : -1;
+        if (r < n_rows) low = min(low, w.lim[t]);
+    }
+    low = __reduce_min_sync(0xffffffffu, low) - (TRX_A4_REC - 1);
+    int st = 0;
+    uint32_t phase = 0;
+    for (; u < n_units; u += step) {
+        if (!__all_sync(0xffffffffu, trx_mbar_wait(&full[warp][st], phase, TRX_WAIT_NS))) break;
+        const int pos = record(u) * TRX_A4_REC;
+        if (pos <= low) w.template record<false>(ring + st * REC, lane, pos);
+        else w.template record<true>(ring + st * REC, lane, pos);
+        __syncwarp();
+        if (lane == 0 && u + S * step < n_units) fetch(u + S * step, st);
+        if (++st == S) st = 0, phase ^= 1;
+    }
+    if (u < n_units && lane == 0) {
+        atomicCAS(err, 0, TRX_A4_GAVE_UP);
+        // (the copies in flight land before the memory is used again)
+        for (int i = 0; i < S && u < n_units; i++, u += step) {
+            trx_mbar_wait(&full[warp][st], phase, TRX_WAIT_NS);
+            if (++st == S) st = 0, phase ^= 1;
+        }
+    }
+    __syncthreads(); // the rings are free
+    float *o = reinterpret_cast<float *>(smem), *refs = o + W * R * HD, *sums = refs + W * R;
+    float *co = reinterpret_cast<float *>(smem + TrxA4Tile<HD, R>::PART), *cref = co + R * HD, *csum = cref + R;
+    w.store(lane, o + warp * R * HD, refs + warp * R, sums + warp * R);
+    __syncthreads();
+    constexpr int ITEMS = R * HD / 4;
+    for (int x = tid; x < ITEMS; x += 32 * W) { // the CTA's warps joined, in their order
+        const int r = x / (HD / 4), d = x % (HD / 4) * 4;
+        float top = refs[r];
+#pragma unroll
+        for (int k = 1; k < W; k++) top = fmaxf(top, refs[k * R + r]);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            const float f = trx_a4_exp2(refs[k * R + r] - top);
+            const float4 y = *reinterpret_cast<const float4 *>(o + (k * R + r) * HD + d);
+            sum = __fmaf_rn(f, sums[k * R + r], sum);
+            v = make_float4(__fmaf_rn(f, y.x, v.x), __fmaf_rn(f, y.y, v.y), __fmaf_rn(f, y.z, v.z), __fmaf_rn(f, y.w, v.w));
+        }
+        if (ranks == 1) {
+            if (r < n_rows)
+                trx_a4_out4<F32>(io, off_o(r) + d, make_float4(__fdiv_rn(v.x, sum), __fdiv_rn(v.y, sum),
+                                                               __fdiv_rn(v.z, sum), __fdiv_rn(v.w, sum)));
+        } else {
+            *reinterpret_cast<float4 *>(co + r * HD + d) = v;
+            if (d == 0) cref[r] = top, csum[r] = sum;
+        }
+    }
+    if (ranks == 1) return;
+    trx_a4_cluster_sync();
+    // the CTAs joined: CTA rank takes an even share of the values, `ranks` neighbouring lanes (a power of two) one of them
+    const int share = ITEMS / ranks, k = tid % ranks;
+    for (int j0 = 0; j0 < share; j0 += 32 * W / ranks) {
+        const int j = j0 + tid / ranks, i = rank * share + min(j, share - 1), r = i / (HD / 4), d = i % (HD / 4) * 4;
+        const float own = trx_a4_peer_load(trx_a4_peer(cref + r, k));
+        float sum = trx_a4_peer_load(trx_a4_peer(csum + r, k));
+        float4 v = trx_a4_peer_load4(trx_a4_peer(co + r * HD + d, k));
+        float top = own;
+        for (int x = 1; x < ranks; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float f = trx_a4_exp2(own - top);
+        sum *= f;
+        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+        for (int x = 1; x < ranks; x <<= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, x);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, x);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, x);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, x);
+        }
+        if (k == 0 && j < share && r < n_rows)
+            trx_a4_out4<F32>(io, off_o(r) + d, make_float4(__fdiv_rn(v.x, sum), __fdiv_rn(v.y, sum),
+                                                           __fdiv_rn(v.z, sum), __fdiv_rn(v.w, sum)));
+    }
+    trx_a4_cluster_sync(); // no CTA leaves while another reads its memory
+}
+
+// The entry a CTA takes in a call of more CTAs than fit at once: the blockIdx.z-th longest, so that the shortest are left
+// for the end (n_entries <= the CTA's threads, all of which call)
+__device__ __forceinline__ int trx_a4_longest(const TrxA4Batch &b, int z) {
+    __shared__ __align__(16) int s_len[32 * TRX_A4_WARPS];
+    __shared__ int s_entry;
+    const int i = threadIdx.x, n = b.n_entries;
+    int len = 0;
+    if (i < n && b.slot[i] >= 0) len = b.pos0[i] + (b.start ? b.start[i + 1] - b.start[i] : 1);
+    s_len[i] = i < n ? len : INT_MIN;
+    __syncthreads();
+    int before = 0;
+    for (int j = 0; j < n; j += 4) {
+        const int4 x = *reinterpret_cast<const int4 *>(s_len + j);
+        before += (x.x > len || (x.x == len && j < i)) + (x.y > len || (x.y == len && j + 1 < i)) +
+                  (x.z > len || (x.z == len && j + 2 < i)) + (x.w > len || (x.w == len && j + 3 < i));
+    }
+    if (i < n && before == z) s_entry = i;
+    __syncthreads();
+    return s_entry;
+}
+
+// blockIdx.x = tile of R rows (token-major, a KV head's query heads side by side; the last tiles, whose contexts are the
+// longest, first) x CTA of the cluster, y the KV head, z the entry
+template <int HD, bool F32, int R>
+__global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
+    trx_a4_attend(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int ranks, int sorted) {
+    extern __shared__ __align__(128) uint8_t smem[];
     int slot, row0, rows, pos0;
-    const int kv = blockIdx.y, r = blockIdx.x, G = a.n_head / a.n_kv;
-    if (!trx_a4_entry(a, b, blockIdx.z, slot, row0, rows, pos0) || r >= rows) return;
-    const uint8_t *recs = a.cache + ((int64_t)slot * a.n_kv + kv) * a.n_blocks * TrxA4L<HD>::REC;
-    const int pos = pos0 + r;
-    for (int h = 0; h < G; h++)
-        trx_a4_attend_row<HD, T>(a, recs, nullptr, pos / TRX_A4_BLOCK + 1, pos,
-                                 q + (int64_t)(row0 + r) * q_stride + (kv * G + h) * HD, scale,
-                                 out + (int64_t)(row0 + r) * out_stride + (kv * G + h) * HD);
+    const int kv = blockIdx.y, G = a.n_head / a.n_kv;
+    const int entry = sorted ? trx_a4_longest(b, blockIdx.z) : blockIdx.z;
+    if (!trx_a4_entry(a, b, entry, slot, row0, rows, pos0)) return;
+    const int total = rows * G, tiles = (total + R - 1) / R, tile = tiles - 1 - (int)(blockIdx.x / ranks);
+    if (tile < 0) return;
+    const uint8_t *recs = a.cache + ((int64_t)slot * a.n_kv + kv) * a.n_blocks * TrxA4L<HD>::BLOCK;
+    const int r0 = tile * R, n_rows = min(R, total - r0), last = pos0 + (r0 + n_rows - 1) / G;
+    auto at = [&](int64_t stride, int r) {
+        const int x = r0 + r, tok = x / G;
+        return (int64_t)(row0 + tok) * stride + (int64_t)(kv * G + x - tok * G) * HD;
+    };
+    trx_a4_tile<HD, F32, R>(
+        smem, a.err, io, recs, nullptr, last / TRX_A4_REC + 1, n_rows, last, scale, ranks,
+        [&](int r) { return pos0 + (r0 + r) / G; }, [&](int r) { return at(io.q_stride, r); },
+        [&](int r) { return at(io.out_stride, r); });
 }
 
 // a float as an unsigned key of the same order (no NaN)
@@ -391,99 +1017,184 @@ __device__ __forceinline__ uint32_t trx_a4_key(float f) {
 // to multiples of a power of two that puts the largest magnitude in [64, 128) and kept within 127. Sums of whole
 // numbers do not depend on their order, so neither does the selection. A block with a NaN among its keys scores +inf;
 // a query with one selects by index. blocks (optional): the selected blocks, ascending, then -1.
-template <int HD, typename T>
-__global__ void __launch_bounds__(256) trx_a4_select(TrxA4 a, TrxA4Batch b, const T *__restrict__ q, int64_t q_stride,
-                                                     float scale, int n_sel, T *__restrict__ out, int64_t out_stride,
-                                                     int32_t *__restrict__ blocks) {
-    constexpr int L = HD / 8;
-    extern __shared__ uint32_t s_key[]; // [n_blocks] keys, then [n_sel] selected blocks
-    __shared__ int s_p[HD], s_n[HD], s_cnt, s_wsum[8];
-    __shared__ float s_max;
+//
+// A cluster shares a (row, KV head): each CTA scores an even part of the earlier blocks (a warp a block: 2 HD bytes, dp2a,
+// one warp reduction) and keeps the keys in shared memory; the threshold is found 8 bits at a time from the CTAs' joined
+// histograms; each CTA sends its selected blocks to every CTA's list, and the cluster attends to the list.
+// blockIdx.x = (row x tiles of R heads) x CTA of the cluster, y the KV head, z the entry. Dynamic shared memory: the
+// tile's (the keys take its place before it starts), at least keys x 4 bytes, then n_sel ints (list_at).
+template <int HD, bool F32, int R>
+__global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
+    trx_a4_select(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int n_sel, int32_t *__restrict__ blocks, int ranks,
+                  int list_at) {
+    constexpr int W = TRX_A4_WARPS, N = 32 * W, PW = HD / 64; // words of bounds a lane takes of a block
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int16_t s_pn[2 * HD]; // N, then P, as the bounds
+    __shared__ int s_hist[4][256], s_warp[2][W], s_cnt[2], s_pick[2], s_before[2];
     int slot, row0, rows, pos0;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = blockIdx.y, r = blockIdx.x, G = a.n_head / a.n_kv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = blockIdx.y, G = a.n_head / a.n_kv;
+    const int tiles = (G + R - 1) / R, r = (int)(blockIdx.x / ranks) / tiles, h0 = (int)(blockIdx.x / ranks) % tiles * R;
     if (!trx_a4_entry(a, b, blockIdx.z, slot, row0, rows, pos0) || r >= rows) return;
-    const int pos = pos0 + r, home = pos / TRX_A4_BLOCK;
+    const int rank = (int)trx_a4_cluster_rank();
+    const int pos = pos0 + r, home = pos / TRX_A4_BLOCK, n_list = min(home + 1, n_sel);
     const int64_t at = ((int64_t)slot * a.n_kv + kv) * a.n_blocks;
-    const T *qr = q + (int64_t)(row0 + r) * q_stride + kv * G * HD;
-    int *list = reinterpret_cast<int *>(s_key + a.n_blocks);
-    int n_list = home + 1;
-    if (n_list > n_sel) {
+    const int64_t qr = (int64_t)(row0 + r) * io.q_stride + (int64_t)kv * G * HD;
+    uint32_t *s_key = reinterpret_cast<uint32_t *>(smem);
+    int *list = reinterpret_cast<int *>(smem + list_at);
+    if (home + 1 > n_sel && n_sel > 1) {
         float most = 0.0f;
         int bad = 0;
-        for (int i = tid; i < G * HD; i += 256) {
-            const float f = fabsf((float)qr[i]);
+        for (int i = tid; i < G * HD; i += N) {
+            const float f = fabsf(trx_a4_q1<F32>(io, qr + i));
             bad |= !(f <= 3.402823466e38f);
             most = fmaxf(most, f);
         }
-        bad = __syncthreads_or(bad);
+        for (int i = tid; i < 4 * 256; i += N) (&s_hist[0][0])[i] = 0;
         for (int s = 16; s; s >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, s));
-        if (lane == 0) s_wsum[warp] = __float_as_int(most);
-        __syncthreads();
-        if (tid == 0) {
-            for (int i = 1; i < 8; i++) most = fmaxf(most, __int_as_float(s_wsum[i]));
-            s_max = most;
-        }
-        __syncthreads();
-        most = s_max;
+        if (lane == 0) s_warp[0][warp] = __float_as_int(most);
+        bad = __syncthreads_or(bad);
+        most = 0.0f;
+        for (int i = 0; i < W; i++) most = fmaxf(most, __int_as_float(s_warp[0][i]));
         if (tid < HD) {
             int ex = 0, up = 0, down = 0;
             if (most > 0.0f && !bad) frexpf(most, &ex);
             for (int h = 0; h < G; h++) {
-                const float f = (float)qr[h * HD + tid];
+                const float f = trx_a4_q1<F32>(io, qr + h * HD + tid);
                 const int z = bad ? 0 : (int)fminf(fmaxf(rintf(ldexpf(f, 7 - ex)), -127.0f), 127.0f);
                 up += max(z, 0);
                 down += min(z, 0);
             }
-            s_p[tid] = up, s_n[tid] = down;
+            s_pn[tid] = (int16_t)down, s_pn[HD + tid] = (int16_t)up;
         }
         __syncthreads();
-        const int l = tid % L;
-        for (int i0 = 0; i0 < home; i0 += 256 / L) {
-            const int i = i0 + tid / L;
-            int sum = 0;
-            if (i < home) {
-                const int8_t *w = a.bounds + (at + i) * (2 * HD) + l * 16;
-                for (int j = 0; j < 8; j++) sum += s_n[8 * l + j] * w[j] + s_p[8 * l + j] * w[8 + j];
+        const int per = (home + ranks - 1) / ranks, base = rank * per, cnt = max(0, min(per, home - base));
+        int pn[2 * PW];
+#pragma unroll
+        for (int i = 0; i < 2 * PW; i++) pn[i] = reinterpret_cast<const int *>(s_pn)[lane * (2 * PW) + i];
+        const int8_t *bounds = a.bounds + (at + base) * (2 * HD);
+        for (int g = warp * 8; g < cnt; g += W * 8) { // 8 blocks in flight
+            int w[8][PW], mine = 0;
+            float u = 0.0f;
+            if (lane < 8 && g + lane < cnt) u = a.units[at + base + g + lane];
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int x = 0; x < PW; x++) w[i][x] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (g + i < cnt) {
+                    const int8_t *p = bounds + (int64_t)(g + i) * (2 * HD) + lane * (4 * PW);
+                    if constexpr (PW == 2) {
+                        const int2 v = *reinterpret_cast<const int2 *>(p);
+                        w[i][0] = v.x, w[i][1] = v.y;
+                    } else w[i][0] = *reinterpret_cast<const int *>(p);
+                }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                int sum = 0;
+#pragma unroll
+                for (int x = 0; x < PW; x++) sum = __dp2a_hi(pn[2 * x + 1], w[i][x], __dp2a_lo(pn[2 * x], w[i][x], sum));
+                sum = __reduce_add_sync(0xffffffffu, sum);
+                if (lane == i) mine = sum;
             }
-            for (int s = 1; s < L; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-            if (i < home && l == 0) {
-                const float u = a.units[at + i];
-                s_key[i] = trx_a4_key(u == INFINITY ? INFINITY : __fmul_rn((float)sum, u));
-            }
+            if (lane < 8 && g + lane < cnt) s_key[g + lane] = trx_a4_key(u == INFINITY ? INFINITY : __fmul_rn((float)mine, u));
         }
         __syncthreads();
-        // the largest key that at least want blocks reach
-        const int want = n_sel - 1;
-        uint32_t t = 0;
-        for (int bit = 31; bit >= 0; bit--) {
-            const uint32_t c = t | (1u << bit);
+        // the largest key that at least n_sel - 1 blocks reach, and how many of the blocks at that key are taken
+        uint32_t key = 0;
+        int want = n_sel - 1;
+        for (int pass = 0; pass < 4; pass++) {
+            const int shift = 24 - 8 * pass;
+            const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
+            for (int i0 = 0; i0 < cnt; i0 += N) {
+                const int i = i0 + tid;
+                const bool on = i < cnt && (s_key[i] & mask) == key;
+                const uint32_t bin = on ? (s_key[i] >> shift) & 255u : 256u;
+                const uint32_t same = __match_any_sync(0xffffffffu, bin); // (most keys share their first bits)
+                if (on && lane == __ffs(same) - 1) atomicAdd(&s_hist[pass][bin], __popc(same));
+            }
+            trx_a4_cluster_sync();
+            int n = 0; // thread: a bin (of 256)
+            if (tid < 256)
+                for (int k = 0; k < ranks; k++) n += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_hist[pass][tid], k)));
+            int above = n; // its blocks and those of the higher bins
+            for (int s = 1; s < 32; s <<= 1) {
+                const int x = __shfl_down_sync(0xffffffffu, above, s);
+                if (lane + s < 32) above += x;
+            }
+            if (lane == 0) s_warp[0][warp] = above;
+            __syncthreads();
+            for (int i = warp + 1; i < W; i++) above += s_warp[0][i];
+            if (above >= want && above - n < want) s_pick[0] = tid, s_pick[1] = want - (above - n);
+            __syncthreads();
+            key |= (uint32_t)s_pick[0] << shift;
+            want = s_pick[1];
+            __syncthreads();
+        }
+        // this CTA's blocks above the key and at it, and those of the CTAs before
+        int above = 0, equal = 0;
+        for (int i = tid; i < cnt; i += N) above += s_key[i] > key, equal += s_key[i] == key;
+        above = __reduce_add_sync(0xffffffffu, above);
+        equal = __reduce_add_sync(0xffffffffu, equal);
+        if (lane == 0) s_warp[0][warp] = above, s_warp[1][warp] = equal;
+        __syncthreads();
+        if (tid < 2) {
             int n = 0;
-            for (int i = tid; i < home; i += 256) n += s_key[i] >= c;
-            if (tid == 0) s_cnt = 0;
+            for (int i = 0; i < W; i++) n += s_warp[tid][i];
+            s_cnt[tid] = n;
+        }
+        trx_a4_cluster_sync();
+        if (tid == 0) {
+            int eq = 0, n = 0;
+            for (int k = 0; k < rank; k++) {
+                n += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_cnt[0], k)));
+                eq += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_cnt[1], k)));
+            }
+            s_before[0] = n + min(eq, want), s_before[1] = eq;
+        }
+        __syncthreads();
+        int place = s_before[0], ties = s_before[1];
+        for (int i0 = 0; i0 < cnt; i0 += N) { // ascending
+            const int i = i0 + tid;
+            const bool eq = i < cnt && s_key[i] == key;
+            const uint32_t e = __ballot_sync(0xffffffffu, eq);
+            if (lane == 0) s_warp[1][warp] = __popc(e);
             __syncthreads();
-            atomicAdd(&s_cnt, n);
+            int before = ties, all = ties;
+            for (int x = 0; x < W; x++) {
+                if (x < warp) before += s_warp[1][x];
+                all += s_warp[1][x];
+            }
+            const bool take = (i < cnt && s_key[i] > key) || (eq && before + __popc(e & ((1u << lane) - 1)) < want);
+            const uint32_t t = __ballot_sync(0xffffffffu, take);
+            if (lane == 0) s_warp[0][warp] = __popc(t);
             __syncthreads();
-            if (s_cnt >= want) t = c;
+            int to = place;
+            for (int x = 0; x < W; x++) {
+                if (x < warp) to += s_warp[0][x];
+                place += s_warp[0][x];
+            }
+            ties = all;
+            if (take) {
+                to += __popc(t & ((1u << lane) - 1));
+                for (int k = 0; k < ranks; k++)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(trx_a4_peer(list + to, k)), "r"(base + i) : "memory");
+            }
             __syncthreads();
         }
-        if (tid == 0) { // ascending: all above t, and the first ones at t
-            int above = 0, n = 0;
-            for (int i = 0; i < home; i++) above += s_key[i] > t;
-            int ties = want - above;
-            for (int i = 0; i < home; i++)
-                if (s_key[i] > t || (s_key[i] == t && ties-- > 0)) list[n++] = i;
-            list[n] = home;
-        }
-        n_list = n_sel;
+        if (tid == 0) list[n_sel - 1] = home;
+        trx_a4_cluster_sync();
     } else {
-        for (int i = tid; i < n_list; i += 256) list[i] = i;
+        for (int i = tid; i < n_list; i += N) list[i] = n_sel == 1 ? home : i;
     }
+    trx_fence_proxy_async(); // (the keys' place becomes the ring)
     __syncthreads();
-    if (blocks)
-        for (int i = tid; i < n_sel; i += 256)
+    if (blocks && h0 == 0 && rank == 0)
+        for (int i = tid; i < n_sel; i += N)
             blocks[((int64_t)(row0 + r) * a.n_kv + kv) * n_sel + i] = i < n_list ? list[i] : -1;
-    const uint8_t *recs = a.cache + at * TrxA4L<HD>::REC;
-    for (int h = 0; h < G; h++)
-        trx_a4_attend_row<HD, T>(a, recs, list, n_list, pos, qr + h * HD, scale,
-                                 out + (int64_t)(row0 + r) * out_stride + (kv * G + h) * HD);
+    const uint8_t *recs = a.cache + at * TrxA4L<HD>::BLOCK;
+    const int64_t outr = (int64_t)(row0 + r) * io.out_stride + (int64_t)kv * G * HD;
+    trx_a4_tile<HD, F32, R>(
+        smem, a.err, io, recs, list, 2 * (n_list - 1) + (pos % TRX_A4_BLOCK) / TRX_A4_REC + 1, min(R, G - h0), pos, scale,
+        ranks, [&](int) { return pos; }, [&](int x) { return qr + (h0 + x) * HD; }, [&](int x) { return outr + (h0 + x) * HD; });
 }
