@@ -66,7 +66,7 @@ def attention(q, k, v, scale, seen=None):
         size = np.where(seen[:, None, :], size, 0)
     p = np.exp(s - s.max(-1, keepdims=True))
     p /= p.sum(-1, keepdims=True)
-    return np.einsum("hgt,thd->hgd", p, v).reshape(q.shape), float(size.max())
+    return np.einsum("hgt,thd->hgd", p, v).reshape(q.shape), float(np.nanmax(size))
 
 
 def tolerance(size, v, out, kind):
@@ -78,9 +78,10 @@ def tolerance(size, v, out, kind):
     the values' largest magnitude. The sums over positions add 2^-24 a position at most, at most 2^12 of them here one
     after another: 2^-12 in the worst case, and their roundings' mean is 0: 2^-17 bounds 64 standard deviations.
     The 16-bit types: a probability times a scale is rounded twice to 16 bits (2 x 2^-11), the minimum's term once, and
-    the result once by half a step of the type."""
-    big = float(abs(v).max())
+    the result once by half a step of the type. Prompts round the keys and the values themselves to 16 bits: 2^-11 x size
+    in a score, and once more on the values."""
+    big = float(np.nanmax(abs(v)))
     tol = 2 * big * (size * (164 / 2 ** 24 + 2 ** -23) + 2 ** -21) + big * 2 ** -17
     if kind != "f32":
-        tol += big * 4 * 2 ** -11 + abs(out) * (2 ** -8 if kind == "bf16" else 2 ** -11)
+        tol += 2 * big * size * 2 ** -11 + big * 4 * 2 ** -11 + abs(out) * (2 ** -8 if kind == "bf16" else 2 ** -11)
     return tol + 1e-30

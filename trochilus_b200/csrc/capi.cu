@@ -33,6 +33,7 @@
 #include "attention.cuh"
 #include "attention4.cuh"
 #include "prefill.cuh"
+#include "attention4_prompt.cuh"
 #include "ep.cuh"
 #include "ffn_norm.cuh"
 
