@@ -3,13 +3,18 @@
 //
 // A CTA takes 256 query rows of a KV head as two tiles of 128 (rows token-major, the KV head's query heads side by
 // side), and all positions they see, 128 at a time:
-//   warps 8-11   read a tile's records and write keys and values as f16, f16(m + d code), into shared memory (K-major,
-//                128-byte swizzle, two stages each): keys [pos][dim], in a record's word order (dims 0 4 1 5 2 6 3 7 of
-//                each 8, the queries' too), values transposed [dim][pos] (a record's words hold position pairs)
-//   warp 12      one thread issues tcgen05.mma (kind::f16, f32 accumulators in tensor memory): S = Q K^T and O += P V, the
+//   warps 8-14   read a tile's records and write values (8-11) and keys (12-14) as f16, f16(m + d code), into shared
+//                memory (K-major, 128-byte swizzle, two stages each), 8 positions of 512 contiguous bytes of codes at a
+//                time, each loaded a tile ahead. Keys [pos][dim] in the order of a lane's words (below: trx_a4p_key), the
+//                queries' too; values transposed [dim][pos]: a lane's pairs of positions are the fragments that stmatrix
+//                stores as rows, dim 32 g + 4 n + i in row 32 g + 8 i + n (O's columns are put right at the end)
+//   warp 15      one thread issues tcgen05.mma (kind::f16, f32 accumulators in tensor memory): S = Q K^T and O += P V, the
 //                tiles in turn, so that one's products run under the other's softmax
-//   warps 0-7    a thread a row: the maximum, 2^(s - ref) as f16 back into tensor memory (P takes S's place), the sum. O
-//                is rescaled only when a row's maximum passes its reference by 2^8 (p stays below 2^15).
+//   warps 0-7    a thread a row, 32 scores at a time: 2^(s - ref) as f16 back into tensor memory (P takes S's place) and
+//                their sum, against the reference of the scores before; where one passes it by 2^8, the references of
+//                the warp's rows move up and O, P and the sums so far are rescaled (p stays below 2^15)
+// The loops are kept short: with all of them unrolled the warps waited for instructions (2 x 2048 rows of 32 heads at 4096
+// positions: 480 us, rolled 320).
 // Tensor memory: S 0, S 1, O 0, O 1, 128 columns each (O: HD).
 //
 // The keys' and values' rounding to f16 (2^-12 relative) is the choice that the 16-bit rows allow: half a step of f16
@@ -21,7 +26,7 @@
 #include "attention4.cuh"
 #include "prefill.cuh"
 
-#define TRX_A4P_THREADS 416
+#define TRX_A4P_THREADS 512
 #define TRX_A4P_ROWS 256 // query rows a CTA
 #define TRX_A4P_KEYS 128 // positions a tile
 
@@ -49,22 +54,68 @@ __device__ __forceinline__ void trx_a4p_mma_ts(uint32_t d, uint32_t a, uint64_t 
                  "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
                  : "memory");
 }
-__device__ __forceinline__ void trx_a4p_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-                 "%15, %16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-                 : "memory");
-}
 __device__ __forceinline__ void trx_a4p_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(trx_smem(bar)) : "memory");
 }
 __device__ __forceinline__ void trx_a4p_inval(uint64_t *bar) {
     asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(trx_smem(bar)) : "memory");
 }
-// a scale's or minimum's |m| + 15 d past what the f16 tiles take (false where d is NaN)
-__device__ __forceinline__ bool trx_a4p_wide(uint32_t d, uint32_t m) {
-    const float2 x = trx_a4_float2(d), y = trx_a4_float2(m);
-    return fmaxf(__fmaf_rn(x.x, 15.0f, fabsf(y.x)), __fmaf_rn(x.y, 15.0f, fabsf(y.y))) > 60000.0f;
+// 32 columns of this warp's rows, in flight until the wait names them
+__device__ __forceinline__ void trx_a4p_landed(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                   "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                   "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void trx_a4p_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                 "%15, %16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+                 "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
+}
+// four 8 x 8 matrices of f16 fragments to shared memory, a row of 16 bytes at each lane's address (lanes 8 i .. 8 i + 7:
+// matrix i)
+__device__ __forceinline__ void trx_a4p_stmatrix(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+// the 16-byte chunk of a key's or query's row that holds dims 32 g + 8 c + 0 4 1 5 2 6 3 7 (eight lanes store the chunks
+// c of one g of two neighbouring rows at a time: these fall into different banks)
+__device__ __forceinline__ int trx_a4p_key(int g, int c) { return (g >> 1) * 8 + 2 * c + (g & 1); }
+// What the f16 tiles do not take: group ends past 60000 (hi: the largest m + 15 d, a NaN stays; lo: the smallest m)
+__device__ __forceinline__ void trx_a4p_ends(uint32_t d, uint32_t m, uint32_t &hi, uint32_t &lo) {
+    asm("{\n .reg .b32 t;\n fma.rn.f16x2 t, %2, %4, %3;\n max.NaN.f16x2 %0, %0, t;\n min.f16x2 %1, %1, %3;\n}"
+        : "+r"(hi), "+r"(lo)
+        : "r"(d), "r"(m), "r"(0x4b804b80u)); // 15
+}
+__device__ __forceinline__ bool trx_a4p_wide(uint32_t hi, uint32_t lo) {
+    const float2 h = trx_a4_float2(hi), l = trx_a4_float2(lo);
+    return h.x > 60000.0f || h.y > 60000.0f || l.x < -60000.0f || l.y < -60000.0f;
+}
+
+// Every row of the warp times its f: n columns of 32-bit floats at `to`, m columns of f16 pairs at `tp`
+__device__ __noinline__ void trx_a4p_rescale(uint32_t to, int n, uint32_t tp, int m, float f) {
+    const uint32_t h = trx_a4_half2(f, f);
+#pragma unroll 1
+    for (int i = 0; i < n; i += 16) {
+        uint32_t r[16];
+        trx_tmem_ld16_nw(to + i, r);
+        trx_tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k++) asm volatile("mul.rn.f32 %0, %0, %1;" : "+r"(r[k]) : "r"(__float_as_uint(f)));
+        trx_a4p_st16(to + i, r);
+    }
+#pragma unroll 1
+    for (int i = 0; i < m; i += 16) {
+        uint32_t r[16];
+        trx_tmem_ld16_nw(tp + i, r);
+        trx_tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 16; k++) asm volatile("mul.rn.f16x2 %0, %0, %1;" : "+r"(r[k]) : "r"(h));
+        trx_a4p_st16(tp + i, r);
+    }
+    trx_tmem_wait_st();
 }
 
 struct TrxA4PBars {
@@ -129,8 +180,9 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
         int ex = 0;
         if (!bad && most > 0.0f) ex = max((int)((__float_as_uint(most) >> 23) & 255) - 126, -100);
         const float f = __int_as_float((10 - ex + 127) << 23) * (scale < 0.0f ? -1.0f : 1.0f);
+        // (kept above 0 and in range: a masked score, -inf, stays one and a score of 0 stays 0)
         c0 = bad ? __int_as_float(0x7fffffff)
-                 : fminf(fabsf(scale) * 1.44269504088896341f * __int_as_float((min(ex, 120) - 10 + 127) << 23), 3.0e36f);
+                 : fminf(1.0e-30f + fabsf(scale) * 1.44269504088896341f * __int_as_float((min(ex, 120) - 10 + 127) << 23), 3.0e36f);
 #pragma unroll
         for (int i = 0; i < HD / 8; i++) { // (dims 32 g + 8 c ..: chunk 4 g + c)
             const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -141,12 +193,12 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                                          : trx_a4_float2(u[j]);
                 x[2 * j] = bad ? 0.0f : y.x * f, x[2 * j + 1] = bad ? 0.0f : y.y * f;
             }
-            *reinterpret_cast<uint4 *>(sq + t_mine * S::Q + trx_a4p_chunk(row, i, 128)) =
+            *reinterpret_cast<uint4 *>(sq + t_mine * S::Q + trx_a4p_chunk(row, trx_a4p_key(i >> 2, i & 3), 128)) =
                 make_uint4(trx_a4_half2(x[0], x[4]), trx_a4_half2(x[1], x[5]), trx_a4_half2(x[2], x[6]), trx_a4_half2(x[3], x[7]));
         }
         trx_fence_proxy_async();
     }
-    if (warp == 12) {
+    if (warp == 15) {
         trx_tmem_alloc(&s_tmem, 512);
         trx_tmem_relinquish();
     }
@@ -164,7 +216,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                     trx_a4p_inval(&bar.o_full[i]);
                     if (i == 0) trx_a4p_inval(&bar.done);
                 }
-                trx_mbar_init(&bar.k_full[i], 4), trx_mbar_init(&bar.v_full[i], 4), trx_mbar_init(&bar.p_ready[i], 4);
+                trx_mbar_init(&bar.k_full[i], 3), trx_mbar_init(&bar.v_full[i], 4), trx_mbar_init(&bar.p_ready[i], 4);
                 trx_mbar_init(&bar.k_empty[i], 1), trx_mbar_init(&bar.v_empty[i], 1), trx_mbar_init(&bar.s_full[i], 1);
                 trx_mbar_init(&bar.o_full[i], 1);
                 if (i == 0) trx_mbar_init(&bar.done, 1);
@@ -187,182 +239,196 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
             const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + 128 * t_mine, to = ts + 256;
             const float c = fminf(c0 * __int_as_float((ek + 127) << 23), 3.0e38f);
             float top = -1.0e30f, ref = -1.0e30f;
-            l = 0.0f;
+            trx_f2 sum = 0;
             const int low = __reduce_min_sync(0xffffffffu, lim);
             for (int j = 0; j < n; j++) {
                 if (!__all_sync(0xffffffffu, wait(&bar.s_full[t_mine], j))) break;
                 trx_tc_fence_after();
                 const bool mask = j * KT + KT - 1 > low;
                 const int see = lim - j * KT; // the tile's last column that the row sees
-                float s[32], best = -INFINITY;
-#pragma unroll 1
-                for (int h = 0; h < 4; h++) {
-                    trx_tmem_ld32(ts + 32 * h, s);
+                // 32 columns from `at`: their maximum, and p
+                auto look = [&](uint32_t(&r)[32], int at) {
                     if (mask) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) s[i] = 32 * h + i > see ? -INFINITY : s[i];
+                        for (int i = 0; i < 32; i++) // (volatile: a branch, not 32 selections for every tile)
+                            asm volatile("{\n .reg .pred q;\n setp.gt.s32 q, %1, %2;\n @q mov.b32 %0, 0xff800000;\n}"
+                                         : "+r"(r[i])
+                                         : "r"(at + i), "r"(see));
                     }
+                    float best[4];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) best = trx_a4_max3(best, s[i], s[i + 1]);
-                }
-                best *= c;
-                if (__any_sync(0xffffffffu, best > top + 8.0f)) { // (S j is complete, so O's products before it are)
-                    top = fmaxf(top, best);
-                    const float next = top == -1.0e30f ? -1.0e30f : top - 7.0f, f = ref == next ? 1.0f : trx_a4_exp2(ref - next);
-                    ref = next;
-                    l *= f;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int h = 0; h < HD / 32; h++) {
-                            trx_tmem_ld32(to + 32 * h, s);
+                    for (int k = 0; k < 4; k++) {
+                        best[k] = fmaxf(__uint_as_float(r[8 * k]), __uint_as_float(r[8 * k + 1]));
 #pragma unroll
-                            for (int i = 0; i < 32; i++) s[i] *= f;
-                            trx_tmem_st32(to + 32 * h, s);
-                        }
-                        trx_tmem_wait_st();
+                        for (int i = 2; i < 8; i += 2)
+                            best[k] = trx_a4_max3(best[k], __uint_as_float(r[8 * k + i]), __uint_as_float(r[8 * k + i + 1]));
                     }
-                }
-                trx_f2 sum = 0;
-#pragma unroll 1
-                for (int h = 0; h < 4; h++) {
-                    trx_tmem_ld32(ts + 32 * h, s);
+                    return trx_a4_max3(fmaxf(best[0], best[1]), best[2], best[3]) * c;
+                };
+                auto take = [&](uint32_t(&r)[32], float best, int at) {
+                    if (__any_sync(0xffffffffu, best > top + 8.0f)) { // (S j is complete: so are O's products before it)
+                        top = fmaxf(top, best);
+                        const float next = top == -1.0e30f ? -1.0e30f : top - 7.0f, f = ref == next ? 1.0f : trx_a4_exp2(ref - next);
+                        ref = next;
+                        sum = trx_mul2(sum, trx_pack2(f, f));
+                        trx_a4p_rescale(to, j > 0 ? HD : 0, ts, at / 2, f);
+                    }
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
-                        float x = trx_a4_exp2(__fmaf_rn(s[i], c, -ref)), y = trx_a4_exp2(__fmaf_rn(s[i + 1], c, -ref));
-                        if (mask) {
-                            if (32 * h + i > see) x = 0.0f;
-                            if (32 * h + i + 1 > see) y = 0.0f;
-                        }
+                        const trx_f2 e = trx_fma2((trx_f2)r[i] | (trx_f2)r[i + 1] << 32, trx_pack2(c, c), trx_pack2(-ref, -ref));
+                        const float x = trx_a4_exp2(trx_lo(e)), y = trx_a4_exp2(trx_hi(e));
                         p[i / 2] = trx_a4_half2(x, y);
                         asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(trx_pack2(x, y)));
                     }
-                    trx_a4p_st16(ts + 16 * h, p); // (S's columns 16 h .. have been read)
+                    trx_a4p_st16(ts + at / 2, p); // (S's columns at / 2 .. have been read)
+                };
+                uint32_t r0[32], r1[32];
+                trx_tmem_ld32_nw(ts, r0);
+                trx_a4p_landed(r0);
+#pragma unroll 1
+                for (int h = 0; h < 128; h += 64) { // (the next 32 are on their way while 32 are taken)
+                    trx_tmem_ld32_nw(ts + h + 32, r1);
+                    float best = look(r0, h);
+                    take(r0, best, h);
+                    trx_a4p_landed(r1);
+                    if (h == 0) trx_tmem_ld32_nw(ts + 64, r0);
+                    best = look(r1, h + 32);
+                    take(r1, best, h + 32);
+                    trx_a4p_landed(r0);
                 }
-                l += trx_lo(sum) + trx_hi(sum);
                 trx_tmem_wait_st();
                 trx_tc_fence_before();
                 __syncwarp();
                 if (lane == 0) trx_a4p_arrive(&bar.p_ready[t_mine]);
             }
+            l = trx_lo(sum) + trx_hi(sum);
             if (n > 0) __all_sync(0xffffffffu, wait(&bar.o_full[t_mine], 0));
             trx_tc_fence_after();
         } else if (warp < 12) {
-            // ---- keys and values to f16
-            const int p = tid - 256;                                          // the key of a tile
-            const int t8 = (lane & 7) + 8 * (warp & 1), vn = (lane >> 3) + 4 * ((warp - 8) >> 1); // 8 positions, dims 32 g + 4 vn ..
-            const __half2 fk = __half2half2(__ushort_as_half((uint16_t)((15 - ek) << 10)));
+            // ---- values to f16: 16 times 8 positions, four a warp; lane (n, c): positions 2 c, 2 c + 1, dims 32 g + 4 n ..
+            struct Piece {
+                uint32_t w[NG], d[NG], m[NG];
+            } first, second;
             const __half2 fv = __half2half2(__ushort_as_half((uint16_t)((15 - ev) << 10)));
-            const uint32_t hk = *reinterpret_cast<const uint32_t *>(&fk), hv = *reinterpret_cast<const uint32_t *>(&fv);
-            bool go = true;
-            for (int j = 0; j < n_all && go; j++) {
-                const int st = j & 1;
-                {
-                    const int pos = j * KT + p;
-                    const uint8_t *rec = recs + (int64_t)(pos >> 5) * REC;
-                    uint32_t w[4][NG], d[NG / 2], m[NG / 2];
+            const uint32_t hv = *reinterpret_cast<const uint32_t *>(&fv);
+            const int cc = lane & 3, t0 = warp - 8; // 8 positions t0 + 4 q: the q-th record's t0-th
+            auto load = [&](Piece &x, int pos) {
+                const uint8_t *rec = recs + (int64_t)(pos >> 5) * REC;
+                if (pos <= last) {
+                    trx_a4_lds<NG>(rec + L::V + t0 * (4 * HD) + lane * (NG * 4), x.w);
+                    trx_a4_lds<NG>(rec + L::VD + (4 * t0 + cc) * (NG * 4), x.d);
+                    trx_a4_lds<NG>(rec + L::VM + (4 * t0 + cc) * (NG * 4), x.m);
+                } else
 #pragma unroll
-                    for (int i = 0; i < NG / 2; i++) d[i] = m[i] = 0;
+                    for (int g = 0; g < NG; g++) x.w[g] = x.d[g] = x.m[g] = 0;
+            };
+            // stmatrix: lane 8 i + n stores the row of dim 32 g + 4 n + i
+            const uint32_t rows = trx_smem(sv) + (lane >> 3) * 1024 + (lane & 7) * 128;
+            auto convert = [&](Piece &x, int pos, int st, int t8) {
+                if (pos + 7 > last) { // (the record's later positions)
+                    const int at = pos + 2 * cc;
+                    const uint32_t on = (at <= last ? 0xffffu : 0u) | (at + 1 <= last ? 0xffff0000u : 0u);
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int g = 0; g < NG; g++) w[i][g] = 0;
-                    if (pos <= last) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) trx_a4_lds<NG>(rec + (pos & 31) * (HD / 2) + i * (NG * 4), w[i]);
-                        trx_a4_lds<NG / 2>(rec + L::KD + (pos & 31) * (NG * 2), d);
-                        trx_a4_lds<NG / 2>(rec + L::KM + (pos & 31) * (NG * 2), m);
-                    }
-                    bool wide = false;
-#pragma unroll
-                    for (int i = 0; i < NG / 2; i++) {
-                        wide |= trx_a4p_wide(d[i], m[i]);
-                        d[i] = trx_a4_hmul2(d[i], hk), m[i] = trx_a4_hmul2(m[i], hk);
-                    }
-                    if (wide) *(volatile int *)&s_wide = 1;
-                    if (j >= 2) go = __all_sync(0xffffffffu, wait(&bar.k_empty[st], (j >> 1) - 1));
-                    if (!go) break;
-                    uint8_t *to = sk + st * S::K;
-#pragma unroll
-                    for (int g = 0; g < NG; g++) {
-                        const uint32_t dd = __byte_perm(d[g / 2], 0, g & 1 ? 0x3232 : 0x1010), mm = __byte_perm(m[g / 2], 0, g & 1 ? 0x3232 : 0x1010);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            uint32_t h[4];
-                            trx_a4_codes<true>(w[i][g], h);
-                            *reinterpret_cast<uint4 *>(to + trx_a4p_chunk(p, 4 * g + i, KT)) =
-                                make_uint4(trx_a4_hfma2(h[0], dd, mm), trx_a4_hfma2(h[1], dd, mm), trx_a4_hfma2(h[2], dd, mm),
-                                           trx_a4_hfma2(h[3], dd, mm));
-                        }
-                    }
-                    trx_fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) trx_a4p_arrive(&bar.k_full[st]);
+                    for (int g = 0; g < NG; g++) x.d[g] &= on, x.m[g] &= on;
                 }
-                {
-                    const int pos = j * KT + 8 * t8;
-                    const uint8_t *rec = recs + (int64_t)(pos >> 5) * REC;
-                    const int t = (pos & 31) >> 3;
-                    uint32_t w[4][NG], d[4][NG], m[4][NG];
-                    bool wide = false, nan = false;
+                uint32_t hi = 0, lo = 0;
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int g = 0; g < NG; g++) w[i][g] = d[i][g] = m[i][g] = 0;
-                    if (pos <= last) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            trx_a4_lds<NG>(rec + L::V + t * (4 * HD) + (4 * vn + i) * (NG * 4), w[i]);
-                            trx_a4_lds<NG>(rec + L::VD + (4 * t + i) * (NG * 4), d[i]);
-                            trx_a4_lds<NG>(rec + L::VM + (4 * t + i) * (NG * 4), m[i]);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) // (scales are not negative: a NaN's bits are above an infinity's)
-#pragma unroll
-                        for (int g = 0; g < NG; g++) nan |= (d[i][g] & 0xffffu) > 0x7c00u || (d[i][g] >> 16) > 0x7c00u;
-                    if (pos + 7 > last || nan) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int g = 0; g < NG; g++)
-#pragma unroll
-                                for (int o = 0; o < 2; o++) {
-                                    const int at = pos + 2 * i + o;
-                                    const bool bad = ((d[i][g] >> (16 * o)) & 0xffffu) > 0x7c00u;
-                                    if (at <= last && bad) atomicMin(&s_nan[g], at);
-                                    if (at > last || bad) d[i][g] &= o ? 0xffffu : 0xffff0000u, m[i][g] &= o ? 0xffffu : 0xffff0000u;
-                                }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int g = 0; g < NG; g++) {
-                            wide |= trx_a4p_wide(d[i][g], m[i][g]);
-                            d[i][g] = trx_a4_hmul2(d[i][g], hv), m[i][g] = trx_a4_hmul2(m[i][g], hv);
-                        }
-                    if (wide) *(volatile int *)&s_wide = 1;
-                    if (j >= 2) go = __all_sync(0xffffffffu, wait(&bar.v_empty[st], (j >> 1) - 1));
-                    if (!go) break;
-                    uint8_t *to = sv + st * S::K;
+                for (int g = 0; g < NG; g++) trx_a4p_ends(x.d[g], x.m[g], hi, lo);
+                const float2 top = trx_a4_float2(hi);
+                if (top.x != top.x || top.y != top.y) { // a NaN: kept apart, and 0 here (its codes and minimum are 0)
+                    hi = 0;
 #pragma unroll
                     for (int g = 0; g < NG; g++) {
-                        uint32_t x[4][4]; // [dim][position pair]
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            uint32_t h[4];
-                            trx_a4_codes<true>(w[i][g], h);
-#pragma unroll
-                            for (int k = 0; k < 4; k++) x[k][i] = trx_a4_hfma2(h[k], d[i][g], m[i][g]);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            *reinterpret_cast<uint4 *>(to + trx_a4p_chunk(32 * g + 4 * vn + k, t8, HD)) =
-                                make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
+                        for (int o = 0; o < 2; o++) // (scales are not negative: a NaN's bits are above an infinity's)
+                            if (((x.d[g] >> (16 * o)) & 0xffffu) > 0x7c00u) {
+                                atomicMin(&s_nan[g], pos + 2 * cc + o);
+                                x.d[g] &= o ? 0xffffu : 0xffff0000u;
+                            }
+                        trx_a4p_ends(x.d[g], x.m[g], hi, lo);
                     }
+                }
+                if (trx_a4p_wide(hi, lo)) *(volatile int *)&s_wide = 1;
+                const uint32_t to = rows + st * S::K + (t8 >> 3) * (HD * 128) + (((t8 & 7) ^ (lane & 7)) << 4);
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    uint32_t h[4];
+                    trx_a4_codes<true>(x.w[g], h);
+                    if (ev) x.d[g] = trx_a4_hmul2(x.d[g], hv), x.m[g] = trx_a4_hmul2(x.m[g], hv);
+                    trx_a4p_stmatrix(to + g * 4096, trx_a4_hfma2(h[0], x.d[g], x.m[g]), trx_a4_hfma2(h[1], x.d[g], x.m[g]),
+                                     trx_a4_hfma2(h[2], x.d[g], x.m[g]), trx_a4_hfma2(h[3], x.d[g], x.m[g]));
+                }
+            };
+            load(first, 8 * t0);
+            load(second, 32 + 8 * t0);
+#pragma unroll 1
+            for (int j = 0, q = 0; j < n_all;) { // 8 positions, and the 8 a record on
+                if (q == 0 && j >= 2 && !__all_sync(0xffffffffu, wait(&bar.v_empty[j & 1], (j >> 1) - 1))) break;
+                const int pos = j * KT + 32 * q + 8 * t0;
+                convert(first, pos, j & 1, 4 * q + t0);
+                load(first, pos + 64);
+                convert(second, pos + 32, j & 1, 4 * q + 4 + t0);
+                load(second, pos + 96);
+                if ((q += 2) == 4) {
                     trx_fence_proxy_async();
                     __syncwarp();
-                    if (lane == 0) trx_a4p_arrive(&bar.v_full[st]);
+                    if (lane == 0) trx_a4p_arrive(&bar.v_full[j & 1]);
+                    q = 0, j++;
+                }
+            }
+        } else if (warp < 15) {
+            // ---- keys to f16: 16 times 8 positions over three warps; lane (n, c): position n, dims 32 g + 8 c ..
+            struct Piece {
+                uint32_t w[NG], d[NG / 2], m[NG / 2];
+            } first, second;
+            const __half2 fk = __half2half2(__ushort_as_half((uint16_t)((15 - ek) << 10)));
+            const uint32_t hk = *reinterpret_cast<const uint32_t *>(&fk);
+            const int n = lane >> 2, cc = lane & 3, x0 = warp - 12;
+            auto load = [&](Piece &x, int pos) {
+                const uint8_t *rec = recs + (int64_t)(pos >> 5) * REC;
+                if (pos <= last) {
+                    trx_a4_lds<NG>(rec + (pos & 31) * (HD / 2) + cc * (NG * 4), x.w);
+                    trx_a4_lds<NG / 2>(rec + L::KD + (pos & 31) * (NG * 2), x.d);
+                    trx_a4_lds<NG / 2>(rec + L::KM + (pos & 31) * (NG * 2), x.m);
+                } else
+#pragma unroll
+                    for (int g = 0; g < NG; g++) x.w[g] = x.d[g / 2] = x.m[g / 2] = 0;
+            };
+            auto convert = [&](Piece &x, int st, int p) {
+                uint32_t hi = 0, lo = 0;
+#pragma unroll
+                for (int i = 0; i < NG / 2; i++) {
+                    trx_a4p_ends(x.d[i], x.m[i], hi, lo); // (beside a NaN: its scores are NaN)
+                    if (ek) x.d[i] = trx_a4_hmul2(x.d[i], hk), x.m[i] = trx_a4_hmul2(x.m[i], hk);
+                }
+                if (trx_a4p_wide(hi, lo)) *(volatile int *)&s_wide = 1;
+                uint8_t *to = sk + st * S::K;
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    const uint32_t half = g & 1 ? 0x3232 : 0x1010;
+                    const uint32_t d = __byte_perm(x.d[g / 2], 0, half), m = __byte_perm(x.m[g / 2], 0, half);
+                    uint32_t h[4];
+                    trx_a4_codes<true>(x.w[g], h);
+                    *reinterpret_cast<uint4 *>(to + trx_a4p_chunk(p, trx_a4p_key(g, cc), KT)) =
+                        make_uint4(trx_a4_hfma2(h[0], d, m), trx_a4_hfma2(h[1], d, m), trx_a4_hfma2(h[2], d, m), trx_a4_hfma2(h[3], d, m));
+                }
+            };
+            load(first, 8 * x0 + n);
+            load(second, 8 * (x0 + 3) + n);
+#pragma unroll 1
+            for (int j = 0, q = 0; j < n_all;) { // (the last of six is there for warp 12 only)
+                if (q == 0 && j >= 2 && !__all_sync(0xffffffffu, wait(&bar.k_empty[j & 1], (j >> 1) - 1))) break;
+                const int p = 8 * (x0 + 3 * q) + n, next = q < 4 ? j * KT + p + 48 : (j + 1) * KT + 8 * x0 + n;
+                convert(first, j & 1, p);
+                load(first, next);
+                if (p + 24 < KT) convert(second, j & 1, p + 24);
+                load(second, next + 24);
+                if ((q += 2) == 6) {
+                    trx_fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) trx_a4p_arrive(&bar.k_full[j & 1]);
+                    q = 0, j++;
                 }
             }
         } else if (lane == 0) {
@@ -435,14 +501,14 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
             if (lim < 0 || *(volatile int *)&s_fail != 0) continue;
             const float x = lim >= s_nan[g] ? __int_as_float(0x7fffffff) : f;
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-                trx_a4_out4<false>(io, out_at + 32 * g + i, make_float4(o[i] * x, o[i + 1] * x, o[i + 2] * x, o[i + 3] * x));
+            for (int i = 0; i < 8; i++)
+                trx_a4_out4<false>(io, out_at + 32 * g + 4 * i, make_float4(o[i] * x, o[8 + i] * x, o[16 + i] * x, o[24 + i] * x));
         }
         if (tid == 0 && s_fail) atomicCAS(a.err, 0, TRX_A4_GAVE_UP);
     }
     trx_tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 15) {
         trx_tc_fence_after();
         trx_tmem_dealloc(s_tmem, 512);
     }
