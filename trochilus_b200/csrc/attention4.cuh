@@ -982,16 +982,16 @@ __device__ __forceinline__ int trx_a4_longest(const TrxA4Batch &b, int z) {
 }
 
 // blockIdx.x = tile of R rows (token-major, a KV head's query heads side by side; the last tiles, whose contexts are the
-// longest, first) x CTA of the cluster, y the KV head, z the entry
+// longest, first) x KV head x CTA of the cluster, z the entry
 template <int HD, bool F32, int R>
 __global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
     trx_a4_attend(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int ranks, int sorted) {
     extern __shared__ __align__(128) uint8_t smem[];
     int slot, row0, rows, pos0;
-    const int kv = blockIdx.y, G = a.n_head / a.n_kv;
+    const int kv = blockIdx.x / ranks % a.n_kv, G = a.n_head / a.n_kv;
     const int entry = sorted ? trx_a4_longest(b, blockIdx.z) : blockIdx.z;
     if (!trx_a4_entry(a, b, entry, slot, row0, rows, pos0)) return;
-    const int total = rows * G, tiles = (total + R - 1) / R, tile = tiles - 1 - (int)(blockIdx.x / ranks);
+    const int total = rows * G, tiles = (total + R - 1) / R, tile = tiles - 1 - (int)(blockIdx.x / ranks / a.n_kv);
     if (tile < 0) return;
     const uint8_t *recs = a.cache + ((int64_t)slot * a.n_kv + kv) * a.n_blocks * TrxA4L<HD>::BLOCK;
     const int r0 = tile * R, n_rows = min(R, total - r0), last = pos0 + (r0 + n_rows - 1) / G;

@@ -119,9 +119,10 @@ __device__ __noinline__ void trx_a4p_rescale(uint32_t to, int n, uint32_t tp, in
 }
 
 struct TrxA4PBars {
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2], done;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], p_read[2], o_full[2], done;
 };
 
+// blockIdx.x = 256 query rows (the last, whose contexts are the longest, first) x KV head, z the entry
 template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
     trx_a4_prompt(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale) {
     using L = TrxA4L<HD>;
@@ -132,9 +133,9 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
     __shared__ uint32_t s_tmem;
     __shared__ int s_fail, s_wide, s_nan[NG], s_most[2];
     int slot, row0, rows, pos0;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv = blockIdx.y, G = a.n_head / a.n_kv;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv = blockIdx.x % a.n_kv, G = a.n_head / a.n_kv;
     if (!trx_a4_entry(a, b, blockIdx.z, slot, row0, rows, pos0)) return;
-    const int total = rows * G, ctas = (total + TRX_A4P_ROWS - 1) / TRX_A4P_ROWS, cta = ctas - 1 - (int)blockIdx.x;
+    const int total = rows * G, ctas = (total + TRX_A4P_ROWS - 1) / TRX_A4P_ROWS, cta = ctas - 1 - (int)(blockIdx.x / a.n_kv);
     if (cta < 0) return;
     const uint8_t *recs = a.cache + ((int64_t)slot * a.n_kv + kv) * a.n_blocks * L::BLOCK;
     const int r0 = cta * TRX_A4P_ROWS;
@@ -213,12 +214,12 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                 if (attempt) {
                     trx_a4p_inval(&bar.k_full[i]), trx_a4p_inval(&bar.k_empty[i]), trx_a4p_inval(&bar.v_full[i]);
                     trx_a4p_inval(&bar.v_empty[i]), trx_a4p_inval(&bar.s_full[i]), trx_a4p_inval(&bar.p_ready[i]);
-                    trx_a4p_inval(&bar.o_full[i]);
+                    trx_a4p_inval(&bar.o_full[i]), trx_a4p_inval(&bar.p_read[i]);
                     if (i == 0) trx_a4p_inval(&bar.done);
                 }
                 trx_mbar_init(&bar.k_full[i], 3), trx_mbar_init(&bar.v_full[i], 4), trx_mbar_init(&bar.p_ready[i], 4);
                 trx_mbar_init(&bar.k_empty[i], 1), trx_mbar_init(&bar.v_empty[i], 1), trx_mbar_init(&bar.s_full[i], 1);
-                trx_mbar_init(&bar.o_full[i], 1);
+                trx_mbar_init(&bar.o_full[i], 1), trx_mbar_init(&bar.p_read[i], 1);
                 if (i == 0) trx_mbar_init(&bar.done, 1);
             }
             trx_fence_barrier_init();
@@ -435,35 +436,42 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
             // ---- products: O t += P t V of the tile before, then S t = Q t K
             const uint32_t aq = trx_smem(sq), ak = trx_smem(sk), av = trx_smem(sv);
             constexpr uint32_t is = S::IDESC | ((uint32_t)(KT >> 3) << 17), iv = S::IDESC | ((uint32_t)(HD >> 3) << 17);
-            bool go = true;
-            for (int j = 0; j <= n_all && go; j++) {
-                for (int t = 0; t < 2 && go; t++) {
-                    if (j > 0 && j - 1 < n_tiles[t]) {
-                        const int st = (j - 1) & 1;
-                        go = wait(&bar.p_ready[t], j - 1) && wait(&bar.v_full[st], (j - 1) >> 1);
-                        if (!go) break;
-                        trx_tc_fence_after();
+            const uint64_t dq = trx_umma_desc_sw128(aq), dk = trx_umma_desc_sw128(ak), dv = trx_umma_desc_sw128(av);
+            const int n0 = n_tiles[0], n1 = n_tiles[1];
+            auto pv = [&](int t, int n, int j) { // O t += P t V of the tile before
+                if (j == 0 || j > n) return true;
+                const int st = (j - 1) & 1;
+                if (!wait(&bar.p_ready[t], j - 1) || !wait(&bar.v_full[st], (j - 1) >> 1)) return false;
+                trx_tc_fence_after();
+                const uint64_t d = dv + (uint64_t)(st * (S::K >> 4));
 #pragma unroll
-                        for (int k = 0; k < KT / 16; k++)
-                            trx_a4p_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k,
-                                           trx_umma_desc_sw128(av + st * S::K + (k >> 2) * (HD * 128) + 32 * (k & 3)), iv,
-                                           j > 1 || k > 0);
-                        if (j == n_tiles[t]) trx_umma_commit(&bar.o_full[t]);
-                    }
-                    if (j < n_tiles[t]) {
-                        const int st = j & 1;
-                        go = wait(&bar.k_full[st], j >> 1);
-                        if (!go) break;
-                        trx_tc_fence_after();
+                for (int k = 0; k < KT / 16; k++)
+                    trx_a4p_mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, d + (uint64_t)((k >> 2) * (HD * 8) + 2 * (k & 3)), iv,
+                                   j > 1 || k > 0);
+                if (j == n) trx_umma_commit(&bar.o_full[t]);
+                else trx_umma_commit(&bar.p_read[t]);
+                return true;
+            };
+            auto qk = [&](int t, int n, int j) { // S t = Q t K
+                if (j >= n) return true;
+                const int st = j & 1;
+                // (S takes P's place: the products that read P are waited for)
+                if (!wait(&bar.k_full[st], j >> 1) || (j > 0 && !wait(&bar.p_read[t], j - 1))) return false;
+                trx_tc_fence_after();
+                const uint64_t da = dq + (uint64_t)(t * (S::Q >> 4)), db = dk + (uint64_t)(st * (S::K >> 4));
 #pragma unroll
-                        for (int k = 0; k < HD / 16; k++)
-                            trx_a4p_mma(tmem + 128 * t, trx_umma_desc_sw128(aq + t * S::Q + (k >> 2) * (128 * 128) + 32 * (k & 3)),
-                                        trx_umma_desc_sw128(ak + st * S::K + (k >> 2) * (KT * 128) + 32 * (k & 3)), is, k > 0);
-                        trx_umma_commit(&bar.s_full[t]);
-                    }
+                for (int k = 0; k < HD / 16; k++) {
+                    const uint64_t o = (uint64_t)((k >> 2) * (128 * 8) + 2 * (k & 3));
+                    trx_a4p_mma(tmem + 128 * t, da + o, db + o, is, k > 0);
                 }
-                if (!go) break;
+                trx_umma_commit(&bar.s_full[t]);
+                return true;
+            };
+#pragma unroll 1
+            for (int j = 0; j <= n_all; j++) {
+                if (!pv(0, n0, j) || !qk(0, n0, j) || !pv(1, n1, j)) break;
                 if (j > 0) trx_umma_commit(&bar.v_empty[(j - 1) & 1]);
+                if (!qk(1, n1, j)) break;
                 if (j < n_all) trx_umma_commit(&bar.k_empty[j & 1]);
             }
             trx_umma_commit(&bar.done); // no product is in flight when the tensor memory goes
