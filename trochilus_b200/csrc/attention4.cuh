@@ -475,6 +475,10 @@ __device__ __forceinline__ uint32_t trx_a4_hfma2(uint32_t a, uint32_t b, uint32_
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
+// a pair of scales, the NaN among them as 0
+__device__ __forceinline__ uint32_t trx_a4_finite(uint32_t d) {
+    return ((d & 0xffffu) > 0x7c00u ? 0u : d & 0xffffu) | ((d >> 16) > 0x7c00u ? 0u : d & 0xffff0000u);
+}
 // NW consecutive words of shared memory
 template <int NW> __device__ __forceinline__ void trx_a4_lds(const uint8_t *p, uint32_t (&w)[NW]) {
     if constexpr (NW == 4) {
@@ -544,14 +548,16 @@ template <bool F32> __device__ __forceinline__ void trx_a4_out4(const TrxA4Rows 
 }
 
 // The 8 codes of a word as four pairs of f16, in the order of bits 0, 4, 8, 12 of its halves: the integers themselves
-// (EXACT), or c 2^-24, 16 c 2^-24, c 2^-24, 16 c 2^-24
-template <bool EXACT> __device__ __forceinline__ void trx_a4_codes(uint32_t w, uint32_t (&h)[4]) {
+// less MID (EXACT), or c 2^-24, 16 c 2^-24, c 2^-24, 16 c 2^-24
+template <bool EXACT, int MID = 0> __device__ __forceinline__ void trx_a4_codes(uint32_t w, uint32_t (&h)[4]) {
+    static_assert(MID == 0 || MID == 8, "");
     const uint32_t v = w >> 8;
     if constexpr (EXACT) { // 1024 + c and 1024 + 16 c from their bits
-        h[0] = trx_a4_hadd2((w & 0x000f000fu) | 0x64006400u, 0xe400e400u);
-        h[1] = trx_a4_hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u);
-        h[2] = trx_a4_hadd2((v & 0x000f000fu) | 0x64006400u, 0xe400e400u);
-        h[3] = trx_a4_hfma2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd400d400u);
+        constexpr uint32_t a = MID ? 0xe408e408u : 0xe400e400u, b = MID ? 0xd480d480u : 0xd400d400u; // -1024 - MID, -64 - MID
+        h[0] = trx_a4_hadd2((w & 0x000f000fu) | 0x64006400u, a);
+        h[1] = trx_a4_hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, b);
+        h[2] = trx_a4_hadd2((v & 0x000f000fu) | 0x64006400u, a);
+        h[3] = trx_a4_hfma2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, b);
     } else {
         h[0] = w & 0x000f000fu, h[1] = w & 0x00f000f0u, h[2] = v & 0x000f000fu, h[3] = v & 0x00f000f0u;
     }
@@ -559,7 +565,11 @@ template <bool EXACT> __device__ __forceinline__ void trx_a4_codes(uint32_t w, u
 
 // One warp's state for R query rows: NT tiles of 8
 template <int HD, bool F32, int R> struct TrxA4Warp {
+    // f32 rows take the codes as integers, the values' around their middle: the codes' sums and the minima's would else be
+    // far larger than what they leave, and the tensor core's additions do not round (subnormal codes lose 3 to 10 bits
+    // more in them, which 16-bit rows can spare)
     static constexpr bool EXACT = F32;
+    static constexpr int MID = F32 ? 8 : 0;
     static constexpr int NG = HD / 32, NT = R / 8, NB = F32 ? 2 : NT;
     static_assert(R == 8 || (R == 16 && !F32), "8 rows, or 16 of a 16-bit type");
     // scores of 16-bit types may pass the reference by 2^LAZY before the sums are rescaled
@@ -772,7 +782,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
         }
 #pragma unroll
         for (int t = 0; t < 2; t++) { // 16 positions: two tiles of 8
-            uint32_t w[2][NG], d[2][NG], m[2], p[2][NT], pl[2], ok[2][NT];
+            uint32_t w[2][NG], d[2][NG], m[2], ml[2] = {0u, 0u}, p[2][NT], pl[2], ok[2][NT];
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 trx_a4_lds<NG>(rec + L::V + (2 * t + k) * (4 * HD) + lane * (NG * 4), w[k]);
@@ -780,6 +790,14 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 // rows 0 .. NG - 1 of A are the groups' minima, row NG ones
                 m[k] = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VM + (8 * t + 4 * k + cc) * (NG * 4) + n * 4)
                               : n == NG ? 0x3c003c00u : 0u;
+                if constexpr (MID != 0) { // m + 8 d, and (rows n + 8) what its rounding drops
+                    const uint32_t x = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VD + (8 * t + 4 * k + cc) * (NG * 4) + n * 4) : 0u;
+                    const float2 md = trx_a4_float2(m[k]), dd = trx_a4_float2(trx_a4_finite(x));
+                    const float y = __fmaf_rn(dd.x, (float)MID, md.x), z = __fmaf_rn(dd.y, (float)MID, md.y);
+                    m[k] = trx_a4_half2(y, z);
+                    const float2 r = trx_a4_float2(m[k]);
+                    ml[k] = trx_a4_half2(y - r.x, z - r.y);
+                }
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
                     const float x = trx_a4_exp2(s[t][r][2 * k] - ref[r][0]), y = trx_a4_exp2(s[t][r][2 * k + 1] - ref[r][1]);
@@ -798,14 +816,14 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
             }
 #pragma unroll
             for (int r = 0; r < NT; r++) {
-                trx_a4_mma16(accm[r], m[0], 0u, m[1], 0u, p[0][r], p[1][r]);
-                if constexpr (F32) trx_a4_mma16(accm[r], m[0], 0u, m[1], 0u, pl[0], pl[1]);
+                trx_a4_mma16(accm[r], m[0], ml[0], m[1], ml[1], p[0][r], p[1][r]);
+                if constexpr (F32) trx_a4_mma16(accm[r], m[0], ml[0], m[1], ml[1], pl[0], pl[1]);
             }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
                 uint32_t u[4], v[4];
-                trx_a4_codes<EXACT>(w[0][g], u);
-                trx_a4_codes<EXACT>(w[1][g], v);
+                trx_a4_codes<EXACT, MID>(w[0][g], u);
+                trx_a4_codes<EXACT, MID>(w[1][g], v);
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
                     uint32_t b0 = trx_a4_hmul2(p[0][r], d[0][g]), b1 = trx_a4_hmul2(p[1][r], d[1][g]);
@@ -836,7 +854,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 if (n == NG) sums[row] = accm[r][i];
 #pragma unroll
                 for (int g = 0; g < NG; g++) { // dims 32 g + 4 n + 0..3
-                    const float m = __shfl_sync(0xffffffffu, accm[r][i], 4 * g + cc);
+                    const float m = __shfl_sync(0xffffffffu, MID ? accm[r][i] + accm[r][2 + i] : accm[r][i], 4 * g + cc);
                     const float e = EXACT ? 1.0f : 16777216.0f, f = EXACT ? 1.0f : 1048576.0f; // 2^24, 2^20
                     *reinterpret_cast<float4 *>(o + row * HD + 32 * g + 4 * n) =
                         make_float4(__fmaf_rn(acc[g][0][r][i], e, m), __fmaf_rn(acc[g][0][r][2 + i], f, m),
