@@ -134,6 +134,23 @@ __device__ __forceinline__ float trx_a4_max3(float a, float b, float c) {
     return d;
 }
 
+// codes with those whose quotient is next to a border taken exactly (seldom called, and kept out of the loops)
+__device__ __noinline__ uint32_t trx_a4_near(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float m,
+                                             float d, float rd, uint32_t codes) {
+    const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float u = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)) * 15.0f, k = floorf(u);
+        if (fabsf(__fsub_rn(__fsub_rn(u, k), 0.5f)) > 3.0e-5f) continue;
+        const float h = __fmul_rn(__fadd_rn(k, 0.5f), d), s = __fadd_rn(m, h);
+        const float t = __fsub_rn(s, m); // s + lost = m + h
+        const float lost = __fadd_rn(__fsub_rn(m, __fsub_rn(s, t)), __fsub_rn(h, t));
+        const bool up = x[j] > s || (x[j] == s && (lost < 0.0f || (lost == 0.0f && ((int)k & 1))));
+        codes = (codes & ~(15u << (4 * j))) | (uint32_t)((int)k + up) << (4 * j);
+    }
+    return codes;
+}
+
 // The 8 codes (4 bits each, value j at bits 4 j), scale and minimum of 8 values of a group whose other 24 lie in the
 // lanes next to this one (4 aligned lanes a group; the whole warp calls); x becomes what they stand for.
 // Both are taken in 32 bits, and exactly where that may round to another side. (hi - m) / 15 is off by less than 2^-22 of
@@ -181,17 +198,9 @@ __device__ __forceinline__ uint32_t trx_a4_quant(float (&x)[8], uint16_t &d16, u
     }
     codes -= 0x3f400000u; // (the sum of the constants that went in with the codes)
     if (fmaxf(trx_a4_max3(trx_a4_max3(far[0], far[1], far[2]), far[3], far[4]), trx_a4_max3(far[5], far[6], far[7])) > 0.49998f) {
+        codes = trx_a4_near(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], m, d, rd, codes);
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (far[j] > 0.49998f) {
-                const float u = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)) * 15.0f, k = floorf(u);
-                const float h = __fmul_rn(__fadd_rn(k, 0.5f), d), s = __fadd_rn(m, h);
-                const float t = __fsub_rn(s, m); // s + lost = m + h
-                const float lost = __fadd_rn(__fsub_rn(m, __fsub_rn(s, t)), __fsub_rn(h, t));
-                const bool up = x[j] > s || (x[j] == s && (lost < 0.0f || (lost == 0.0f && ((int)k & 1))));
-                q[j] = up ? k + 1.0f : k;
-                codes = (codes & ~(15u << (4 * j))) | (uint32_t)(int)q[j] << (4 * j);
-            }
+        for (int j = 0; j < 8; j++) q[j] = (float)((codes >> (4 * j)) & 15);
     }
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = __fmaf_rn(d, q[j], m); // (d x code is exact)
@@ -468,6 +477,11 @@ __device__ __forceinline__ uint32_t trx_a4_hmul2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t trx_a4_hadd2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t trx_a4_hfms2(uint32_t a, uint32_t b, uint32_t c) { // a b - c
+    uint32_t d;
+    asm("{\n .reg .b32 t;\n neg.f16x2 t, %3;\n fma.rn.f16x2 %0, %1, %2, t;\n}" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
 __device__ __forceinline__ uint32_t trx_a4_hfma2(uint32_t a, uint32_t b, uint32_t c) {
@@ -790,9 +804,10 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 // rows 0 .. NG - 1 of A are the groups' minima, row NG ones
                 m[k] = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VM + (8 * t + 4 * k + cc) * (NG * 4) + n * 4)
                               : n == NG ? 0x3c003c00u : 0u;
-                if constexpr (MID != 0) { // m + 8 d, and (rows n + 8) what its rounding drops
+                // m + 8 d, and (rows n + 8) what its rounding drops; a NaN belongs to every row where all see the position
+                if constexpr (MID != 0) {
                     const uint32_t x = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VD + (8 * t + 4 * k + cc) * (NG * 4) + n * 4) : 0u;
-                    const float2 md = trx_a4_float2(m[k]), dd = trx_a4_float2(trx_a4_finite(x));
+                    const float2 md = trx_a4_float2(m[k]), dd = trx_a4_float2(MASK ? trx_a4_finite(x) : x);
                     const float y = __fmaf_rn(dd.x, (float)MID, md.x), z = __fmaf_rn(dd.y, (float)MID, md.y);
                     m[k] = trx_a4_half2(y, z);
                     const float2 r = trx_a4_float2(m[k]);
@@ -828,8 +843,8 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 for (int r = 0; r < NT; r++) {
                     uint32_t b0 = trx_a4_hmul2(p[0][r], d[0][g]), b1 = trx_a4_hmul2(p[1][r], d[1][g]);
                     if constexpr (F32) { // p d in two parts: what the product's rounding drops, and the lower part's product
-                        uint32_t l0 = trx_a4_hfma2(pl[0], d[0][g], trx_a4_hfma2(p[0][r], d[0][g], b0 ^ 0x80008000u));
-                        uint32_t l1 = trx_a4_hfma2(pl[1], d[1][g], trx_a4_hfma2(p[1][r], d[1][g], b1 ^ 0x80008000u));
+                        uint32_t l0 = trx_a4_hfma2(pl[0], d[0][g], trx_a4_hfms2(p[0][r], d[0][g], b0));
+                        uint32_t l1 = trx_a4_hfma2(pl[1], d[1][g], trx_a4_hfms2(p[1][r], d[1][g], b1));
                         if constexpr (MASK) l0 &= ok[0][r], l1 &= ok[1][r];
                         trx_a4_mma16(acc[g][0][r], u[0], u[1], v[0], v[1], l0, l1);
                         trx_a4_mma16(acc[g][1][r], u[2], u[3], v[2], v[3], l0, l1);
@@ -875,6 +890,10 @@ __device__ __forceinline__ void trx_a4_tile(uint8_t *smem, int32_t *err, const T
     __shared__ __align__(8) uint64_t full[W][S];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = ranks > 1 ? (int)trx_a4_cluster_rank() : 0;
+    if (n_units <= W) { // one CTA's work: the others leave, and nobody meets
+        if (rank > 0) return;
+        ranks = 1;
+    }
     // (a warp uses its own barriers only)
     if (lane == 0) {
         for (int i = 0; i < S; i++) trx_mbar_init(&full[warp][i], 1);
