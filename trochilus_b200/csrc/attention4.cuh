@@ -9,7 +9,7 @@
 // d = NaN, m = 0 and codes 0: it reads back as NaN, and m is always finite.
 //
 // 32 positions of a (layer, sequence, KV head) are one record of contiguous memory (5120 bytes for HD 128: 5 bits a
-// value), one bulk copy of the attention kernel:
+// value):
 //   keys    codes  [pos][c][g] one 32-bit word: dims 32 g + 8 c + j (j = 0..7) at bits 4 j        32 x HD / 2 bytes
 //           d, m   [pos][g] f16
 //   values  codes  [pos / 8][n][c][g][odd] 16 bits (pos % 8 = 2 c + odd): dims 32 g + 4 n + i (i = 0..3) at bits 4 i
@@ -422,11 +422,14 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 // exactly: a word of 8 codes is one shift and four ANDs, and no subtraction of a bias. The query values that meet a
 // 16 c are stored divided by 16; the outputs that come of one are divided by 16 at the end, where 2^24 goes too.
 //
-// A warp takes records of 32 positions through its own ring of two bulk copies, 16 positions at a time:
+// A warp takes records of 32 positions through its own ring of two, 16 positions at a time. (It fills the ring with
+// 16-byte asynchronous copies, a group a record: a bulk copy, which one lane issues, held the warp up for 600 of 2800
+// cycles a record.)
 //   scores   mma m16n8k16: A = 16 keys x 16 codes, B = 8 query rows (f32 rows: a second B with what f16 drops of the
 //            first); a group is two of them, then d; the minima's sums are one m16n8k8 with B = sum_i x_gi in two f16
 //            parts
-//   softmax  running maximum a row; p in f16 (f32 rows: two f16 parts, 22 bits), transposed in registers (movmatrix)
+//   softmax  a reference a row, which moves only when a score passes it (16-bit rows: by 2^8), so that the usual record
+//            needs one vote and no reduction; p in f16 (f32 rows: two f16 parts, 22 bits), transposed in registers (movmatrix)
 //   outputs  mma m16n8k16: A = 16 dims x 16 positions of codes, B = p_t d_tg of 8 rows; one more with the minima (and
 //            ones, which sum p) as A.
 // 16 query rows of f16 or bf16 type, or 8 (R), share the codes' unpacking; scores, sums and outputs are f32.
@@ -734,24 +737,16 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 s[t][r][2] = trx_lo(a[r][1]), s[t][r][3] = trx_hi(a[r][1]);
             }
         }
-        // the largest value scale of the record, where it passes those before
-        bool grow = false;
-        {
-            uint32_t w[NG / 2];
-            trx_a4_lds<NG / 2>(rec + L::VD + lane * (NG * 2), w);
-            float2 f = trx_a4_float2(w[0]);
-            float big = fmaxf(f.x, f.y);
-            if constexpr (NG == 4) {
-                f = trx_a4_float2(w[NG / 2 - 1]);
-                big = fmaxf(big, fmaxf(f.x, f.y));
-            }
-            if (__any_sync(0xffffffffu, big > edlim)) {
-                for (int x = 16; x; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-                const int e = (int)((__float_as_uint(big) >> 23) & 255) - 126; // 2^e > big
-                ed = (float)e, edlim = __int_as_float((e + 127) << 23);
-                grow = true;
-            }
+        // does a score pass its row's reference, or a value scale the largest before?
+        uint32_t vd[NG / 2];
+        trx_a4_lds<NG / 2>(rec + L::VD + lane * (NG * 2), vd);
+        float2 e = trx_a4_float2(vd[0]);
+        float big = fmaxf(e.x, e.y);
+        if constexpr (NG == 4) {
+            e = trx_a4_float2(vd[NG / 2 - 1]);
+            big = fmaxf(big, fmaxf(e.x, e.y));
         }
+        bool grow = big > edlim;
         float f[NT][2];
 #pragma unroll
         for (int r = 0; r < NT; r++) {
@@ -768,17 +763,23 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                         if (MASK && pos0 + 16 * t + 8 * k + n > last) x = -INFINITY;
                         best = fmaxf(best, x);
                     }
-#pragma unroll
-                for (int x = 4; x <= 16; x <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
                 grow |= best > top[r][i] + LAZY;
                 f[r][i] = best;
             }
         }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
+            for (int x = 1; x <= 16; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+            if (big > edlim) {
+                const int x = (int)((__float_as_uint(big) >> 23) & 255) - 126; // 2^x > big
+                ed = (float)x, edlim = __int_as_float((x + 127) << 23);
+            }
+#pragma unroll
             for (int r = 0; r < NT; r++) {
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
+#pragma unroll
+                    for (int x = 4; x <= 16; x <<= 1) f[r][i] = fmaxf(f[r][i], __shfl_xor_sync(0xffffffffu, f[r][i], x));
                     top[r][i] = fmaxf(top[r][i], f[r][i]);
                     const float to = top[r][i] == -1.0e30f ? -1.0e30f : top[r][i] + ed - TOP;
                     f[r][i] = ref[r][i] == to ? 1.0f : trx_a4_exp2(ref[r][i] - to);
@@ -881,36 +882,34 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 
 // A tile of query rows (row r: its values at off_q(r) and off_o(r), its last position lim(r)) over the first n_units
 // records (of the listed blocks, or 0, 1, ..), by the CTAs of the cluster (ranks of them). smem: TrxA4Tile::SMEM bytes,
-// 128-byte aligned; no copy may be in flight into it, and what was read of it is ordered before (the caller's barrier).
+// 128-byte aligned; what was read of it is ordered before (the caller's barrier).
 template <int HD, bool F32, int R, typename Lim, typename OffQ, typename OffO>
-__device__ __forceinline__ void trx_a4_tile(uint8_t *smem, int32_t *err, const TrxA4Rows &io, const uint8_t *recs,
+__device__ __forceinline__ void trx_a4_tile(uint8_t *smem, const TrxA4Rows &io, const uint8_t *recs,
                                             const int *list, int n_units, int n_rows, int last, float scale, int ranks,
                                             Lim lim, OffQ off_q, OffO off_o) {
     constexpr int REC = TrxA4L<HD>::REC, S = TRX_A4_STAGES, W = TRX_A4_WARPS;
-    __shared__ __align__(8) uint64_t full[W][S];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = ranks > 1 ? (int)trx_a4_cluster_rank() : 0;
     if (n_units <= W) { // one CTA's work: the others leave, and nobody meets
         if (rank > 0) return;
         ranks = 1;
     }
-    // (a warp uses its own barriers only)
-    if (lane == 0) {
-        for (int i = 0; i < S; i++) trx_mbar_init(&full[warp][i], 1);
-        trx_fence_barrier_init();
-    }
-    __syncwarp();
     uint8_t *ring = smem + warp * (S * REC);
     const int step = ranks * W;
     auto record = [&](int u) { return list ? 2 * list[u >> 1] + (u & 1) : u; }; // the u-th record's index
     auto fetch = [&](int u, int st) {
-        trx_mbar_expect_tx(&full[warp][st], REC);
-        trx_bulk_g2s(ring + st * REC, recs + (int64_t)record(u) * REC, REC, &full[warp][st]);
+        if (u < n_units) {
+            const uint8_t *src = recs + (int64_t)record(u) * REC + lane * 16;
+            const uint32_t dst = trx_smem(ring + st * REC + lane * 16);
+#pragma unroll
+            for (int i = 0; i < REC / 512; i++)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * 512), "l"(src + i * 512) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
     int u = rank * W + warp;
-    if (lane == 0)
-        for (int i = 0; i < S; i++)
-            if (u + i * step < n_units) fetch(u + i * step, i);
+#pragma unroll
+    for (int i = 0; i < S; i++) fetch(u + i * step, i);
     TrxA4Warp<HD, F32, R> w;
     w.load(io, lane, n_rows, scale, off_q);
     int low = last; // the lowest of the rows' last positions
@@ -921,25 +920,17 @@ __device__ __forceinline__ void trx_a4_tile(uint8_t *smem, int32_t *err, const T
         if (r < n_rows) low = min(low, w.lim[t]);
     }
     low = __reduce_min_sync(0xffffffffu, low) - (TRX_A4_REC - 1);
-    int st = 0;
-    uint32_t phase = 0;
-    for (; u < n_units; u += step) {
-        if (!__all_sync(0xffffffffu, trx_mbar_wait(&full[warp][st], phase, TRX_WAIT_NS))) break;
+    for (int st = 0; u < n_units; u += step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(TRX_A4_STAGES - 1) : "memory");
+        __syncwarp();
         const int pos = record(u) * TRX_A4_REC;
         if (pos <= low) w.template record<false>(ring + st * REC, lane, pos);
         else w.template record<true>(ring + st * REC, lane, pos);
         __syncwarp();
-        if (lane == 0 && u + S * step < n_units) fetch(u + S * step, st);
-        if (++st == S) st = 0, phase ^= 1;
+        fetch(u + S * step, st);
+        st = st + 1 == S ? 0 : st + 1;
     }
-    if (u < n_units && lane == 0) {
-        atomicCAS(err, 0, TRX_A4_GAVE_UP);
-        // (the copies in flight land before the memory is used again)
-        for (int i = 0; i < S && u < n_units; i++, u += step) {
-            trx_mbar_wait(&full[warp][st], phase, TRX_WAIT_NS);
-            if (++st == S) st = 0, phase ^= 1;
-        }
-    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads(); // the rings are free
     float *o = reinterpret_cast<float *>(smem), *refs = o + W * R * HD, *sums = refs + W * R;
     float *co = reinterpret_cast<float *>(smem + TrxA4Tile<HD, R>::PART), *cref = co + R * HD, *csum = cref + R;
@@ -1037,7 +1028,7 @@ __global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
         return (int64_t)(row0 + tok) * stride + (int64_t)(kv * G + x - tok * G) * HD;
     };
     trx_a4_tile<HD, F32, R>(
-        smem, a.err, io, recs, nullptr, last / TRX_A4_REC + 1, n_rows, last, scale, ranks,
+        smem, io, recs, nullptr, last / TRX_A4_REC + 1, n_rows, last, scale, ranks,
         [&](int r) { return pos0 + (r0 + r) / G; }, [&](int r) { return at(io.q_stride, r); },
         [&](int r) { return at(io.out_stride, r); });
 }
@@ -1224,14 +1215,13 @@ __global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
     } else {
         for (int i = tid; i < n_list; i += N) list[i] = n_sel == 1 ? home : i;
     }
-    trx_fence_proxy_async(); // (the keys' place becomes the ring)
-    __syncthreads();
+    __syncthreads(); // (the keys' place becomes the ring)
     if (blocks && h0 == 0 && rank == 0)
         for (int i = tid; i < n_sel; i += N)
             blocks[((int64_t)(row0 + r) * a.n_kv + kv) * n_sel + i] = i < n_list ? list[i] : -1;
     const uint8_t *recs = a.cache + at * TrxA4L<HD>::BLOCK;
     const int64_t outr = (int64_t)(row0 + r) * io.out_stride + (int64_t)kv * G * HD;
     trx_a4_tile<HD, F32, R>(
-        smem, a.err, io, recs, list, 2 * (n_list - 1) + (pos % TRX_A4_BLOCK) / TRX_A4_REC + 1, min(R, G - h0), pos, scale,
+        smem, io, recs, list, 2 * (n_list - 1) + (pos % TRX_A4_BLOCK) / TRX_A4_REC + 1, min(R, G - h0), pos, scale,
         ranks, [&](int) { return pos; }, [&](int x) { return qr + (h0 + x) * HD; }, [&](int x) { return outr + (h0 + x) * HD; });
 }
