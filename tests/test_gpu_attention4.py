@@ -181,7 +181,7 @@ def test_quantiser_borders(cuda):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("heads,kv,hd", ((16, 16, 128), (8, 2, 128), (14, 2, 64), (16, 1, 64), (40, 2, 128), (3, 1, 128)))
+@pytest.mark.parametrize("heads,kv,hd", ((16, 16, 128), (8, 2, 128), (14, 2, 64), (16, 1, 64), (40, 2, 128), (3, 1, 128), (256, 1, 64)))
 def test_decode_attention(cuda, kind, heads, kv, hd):
     """one row a sequence, lengths from one position on, in one call"""
     rng = np.random.default_rng(3)
@@ -484,6 +484,72 @@ def test_captured_and_replayed(cuda):
                 assert np.array_equal(blocks[i].cpu().numpy(), orc.selected(s.k[sl], hq, at[i], 4))
     s.s.check()
     s.close(), o.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,hd", ((4, 4, 128), (8, 2, 128), (16, 1, 64), (20, 1, 128)))
+def test_long_contexts(cuda, kind, heads, kv, hd):
+    """many CTAs and warps on one tile of query rows, of which some, most or all but one have a position; drafted tokens;
+    the selection's threshold over several CTAs"""
+    rng = np.random.default_rng(16)
+    ctx = 20001
+    s = Session(cuda, 2, heads, kv, hd, ctx)
+    s.write([(1, 0, ctx)], *_rows(rng, ctx, kv, hd), kind)
+    s.write([(0, 0, 600)], *_rows(rng, 600, kv, hd), kind)
+    q = rng.normal(size=(8, heads, hd)).astype(np.float32)
+    for entries in ([(1, 20000, 1)], [(1, 16383, 1)], [(1, 300, 1)], [(0, 31, 1)], [(0, 599, 1), (1, 9000, 1)], [(1, 19993, 8)]):
+        n = sum(e[2] for e in entries)
+        s.check_attend(entries, q[:n], kind)
+        s.check_attend(entries, q[:n], kind, n_sel=7)
+    s.check_attend([(1, 20000, 1)], q[:1], kind, n_sel=200)
+    s.s.check()
+    s.close()
+
+
+def test_overlapping_calls(cuda):
+    """one session's calls on two streams at once, eager and as two captured graphs: each gives what it gives alone"""
+    torch = cuda
+    rng = np.random.default_rng(17)
+    s = Session(torch, 4, 8, 2, 128, 3000)
+    s.write([(i, 0, 3000) for i in range(4)], *_rows(rng, 12000, 2, 128), "f16")
+    jobs = []
+    for entries in ([(0, 2999, 1), (1, 700, 1)], [(2, 2000, 1), (3, 64, 1), (0, 2998, 1)]):
+        b = s.batch(entries)
+        q = torch.from_numpy(rng.normal(size=(len(entries), 8, 128)).astype(np.float32)).to("cuda").half()
+        jobs.append((b, q, torch.zeros_like(q), torch.zeros_like(q), torch.cuda.Stream()))
+
+    def run(job, stream):
+        b, q, out, picked, _ = job
+        for _ in range(4):
+            s.s.attend_dev(0, b, s.moe.F16, q.data_ptr(), 1024, 0.1, out.data_ptr(), 1024, stream=stream)
+            s.s.select_dev(0, b, s.moe.F16, q.data_ptr(), 1024, 0.1, 5, picked.data_ptr(), 1024, stream=stream)
+
+    alone = []
+    for job in jobs:
+        run(job, torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        alone.append((job[2].clone(), job[3].clone()))
+    graphs = []
+    for job in jobs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(job, torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for it in range(20):
+        for job in jobs:
+            job[2].zero_(), job[3].zero_()
+        torch.cuda.synchronize()
+        for job, g in zip(jobs, graphs):
+            with torch.cuda.stream(job[4]):
+                if it % 2:
+                    g.replay()
+                else:
+                    run(job, job[4].cuda_stream)
+        torch.cuda.synchronize()
+        for job, (out, picked) in zip(jobs, alone):
+            assert torch.equal(job[2], out) and torch.equal(job[3], picked)
+    s.s.check()
+    s.close()
 
 
 def test_far_offsets(cuda):

@@ -439,7 +439,6 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 // A cluster of CTAs shares one tile of query rows: its warps take records in turn, their results are joined in each
 // CTA through shared memory, and the CTAs' through distributed shared memory, so that no workspace or second launch is
 // needed and overlapping calls share nothing.
-#define TRX_A4_WARPS 8
 #define TRX_A4_STAGES 2
 
 __device__ __forceinline__ void trx_a4_mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -532,8 +531,8 @@ __device__ __forceinline__ float trx_a4_peer_load(uint32_t a) {
     return v;
 }
 
-template <int HD, int R> struct TrxA4Tile { // shared memory of a tile of R query rows
-    static constexpr int W = TRX_A4_WARPS, RING = W * TRX_A4_STAGES * TrxA4L<HD>::REC, PARTS = W * R * (HD + 2) * 4;
+template <int HD, int R, int W> struct TrxA4Tile { // shared memory of a tile of R query rows, CTAs of W warps
+    static constexpr int RING = W * TRX_A4_STAGES * TrxA4L<HD>::REC, PARTS = W * R * (HD + 2) * 4;
     static constexpr int PART = RING > PARTS ? RING : PARTS; // the ring, then in its place the warps' results
     static constexpr int SMEM = PART + R * (HD + 2) * 4;     // behind them the CTA's result
 };
@@ -564,20 +563,23 @@ template <bool F32> __device__ __forceinline__ void trx_a4_out4(const TrxA4Rows 
         *reinterpret_cast<uint2 *>((__half *)io.out + at) = make_uint2(trx_a4_half2(v.x, v.y), trx_a4_half2(v.z, v.w));
 }
 
-// The 8 codes of a word as four pairs of f16, in the order of bits 0, 4, 8, 12 of its halves: the integers themselves
-// less MID (EXACT), or c 2^-24, 16 c 2^-24, c 2^-24, 16 c 2^-24
-template <bool EXACT, int MID = 0> __device__ __forceinline__ void trx_a4_codes(uint32_t w, uint32_t (&h)[4]) {
+// The codes at bits 0 and 4 of a word's halves as two pairs of f16: the integers themselves less MID (EXACT), or c 2^-24
+// and 16 c 2^-24. (A word's other four: of the word shifted by 8.)
+template <bool EXACT, int MID = 0> __device__ __forceinline__ void trx_a4_half_codes(uint32_t w, uint32_t (&h)[2]) {
     static_assert(MID == 0 || MID == 8, "");
-    const uint32_t v = w >> 8;
     if constexpr (EXACT) { // 1024 + c and 1024 + 16 c from their bits
         constexpr uint32_t a = MID ? 0xe408e408u : 0xe400e400u, b = MID ? 0xd480d480u : 0xd400d400u; // -1024 - MID, -64 - MID
         h[0] = trx_a4_hadd2((w & 0x000f000fu) | 0x64006400u, a);
         h[1] = trx_a4_hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, b);
-        h[2] = trx_a4_hadd2((v & 0x000f000fu) | 0x64006400u, a);
-        h[3] = trx_a4_hfma2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, b);
     } else {
-        h[0] = w & 0x000f000fu, h[1] = w & 0x00f000f0u, h[2] = v & 0x000f000fu, h[3] = v & 0x00f000f0u;
+        h[0] = w & 0x000f000fu, h[1] = w & 0x00f000f0u;
     }
+}
+template <bool EXACT, int MID = 0> __device__ __forceinline__ void trx_a4_codes(uint32_t w, uint32_t (&h)[4]) {
+    uint32_t a[2], b[2];
+    trx_a4_half_codes<EXACT, MID>(w, a);
+    trx_a4_half_codes<EXACT, MID>(w >> 8, b);
+    h[0] = a[0], h[1] = a[1], h[2] = b[0], h[3] = b[1];
 }
 
 // One warp's state for R query rows: NT tiles of 8
@@ -712,23 +714,31 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                     a[r][0] = trx_mul2(a[r][0], tiny), a[r][1] = trx_mul2(a[r][1], tiny);
                 }
             }
+            // (the groups' products side by side: each waits for the one before it in its group only)
+            float x[NG][NT][4];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int g = 0; g < NG; g++) {
+                    uint32_t u[2], v[2];
+                    trx_a4_half_codes<EXACT>(h ? w0[g] >> 8 : w0[g], u);
+                    trx_a4_half_codes<EXACT>(h ? w1[g] >> 8 : w1[g], v);
+#pragma unroll
+                    for (int r = 0; r < NT; r++) {
+                        if (h == 0) x[g][r][0] = x[g][r][1] = x[g][r][2] = x[g][r][3] = 0.0f;
+#pragma unroll
+                        for (int b = r; b < NB; b += NT)
+                            trx_a4_mma16(x[g][r], u[0], v[0], u[1], v[1], qb[b][2 * g + h][0], qb[b][2 * g + h][1]);
+                    }
+                }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
-                uint32_t u[4], v[4];
-                trx_a4_codes<EXACT>(w0[g], u);
-                trx_a4_codes<EXACT>(w1[g], v);
                 const float2 e0 = trx_a4_float2(d0[g / 2]), e1 = trx_a4_float2(d1[g / 2]);
                 const float f0 = g & 1 ? e0.y : e0.x, f1 = g & 1 ? e1.y : e1.x;
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
-                    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int b = r; b < NB; b += NT) {
-                        trx_a4_mma16(x, u[0], v[0], u[1], v[1], qb[b][2 * g][0], qb[b][2 * g][1]);
-                        trx_a4_mma16(x, u[2], v[2], u[3], v[3], qb[b][2 * g + 1][0], qb[b][2 * g + 1][1]);
-                    }
-                    a[r][0] = trx_fma2(trx_pack2(x[0], x[1]), trx_pack2(f0, f0), a[r][0]);
-                    a[r][1] = trx_fma2(trx_pack2(x[2], x[3]), trx_pack2(f1, f1), a[r][1]);
+                    a[r][0] = trx_fma2(trx_pack2(x[g][r][0], x[g][r][1]), trx_pack2(f0, f0), a[r][0]);
+                    a[r][1] = trx_fma2(trx_pack2(x[g][r][2], x[g][r][3]), trx_pack2(f1, f1), a[r][1]);
                 }
             }
 #pragma unroll
@@ -795,9 +805,24 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                         for (int i = 0; i < 4; i++) acc[g][h][r][i] *= f[r][i & 1];
             }
         }
+        uint32_t ps[4][NT], pls[4]; // 8 positions each
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int r = 0; r < NT; r++) {
+                const float x = trx_a4_exp2(s[k / 2][r][2 * (k & 1)] - ref[r][0]), y = trx_a4_exp2(s[k / 2][r][2 * (k & 1) + 1] - ref[r][1]);
+                const uint32_t h = trx_a4_half2(x, y);
+                ps[k][r] = trx_a4_transpose(h);
+                if constexpr (F32) {
+                    const float2 b = trx_a4_float2(h);
+                    pls[k] = trx_a4_transpose(trx_a4_half2(x - b.x, y - b.y));
+                }
+            }
 #pragma unroll
         for (int t = 0; t < 2; t++) { // 16 positions: two tiles of 8
-            uint32_t w[2][NG], d[2][NG], m[2], ml[2] = {0u, 0u}, p[2][NT], pl[2], ok[2][NT];
+            uint32_t w[2][NG], d[2][NG], m[2], ml[2] = {0u, 0u}, ok[2][NT];
+            const uint32_t(&p)[2][NT] = reinterpret_cast<const uint32_t(&)[2][NT]>(ps[2 * t]);
+            const uint32_t(&pl)[2] = reinterpret_cast<const uint32_t(&)[2]>(pls[2 * t]);
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 trx_a4_lds<NG>(rec + L::V + (2 * t + k) * (4 * HD) + lane * (NG * 4), w[k]);
@@ -816,13 +841,6 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 }
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
-                    const float x = trx_a4_exp2(s[t][r][2 * k] - ref[r][0]), y = trx_a4_exp2(s[t][r][2 * k + 1] - ref[r][1]);
-                    const uint32_t h = trx_a4_half2(x, y);
-                    p[k][r] = trx_a4_transpose(h);
-                    if constexpr (F32) {
-                        const float2 b = trx_a4_float2(h);
-                        pl[k] = trx_a4_transpose(trx_a4_half2(x - b.x, y - b.y));
-                    }
                     // (a masked position's scale may be a NaN)
                     if constexpr (MASK) {
                         const int at = pos0 + 16 * t + 8 * k + 2 * cc;
@@ -883,11 +901,11 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 // A tile of query rows (row r: its values at off_q(r) and off_o(r), its last position lim(r)) over the first n_units
 // records (of the listed blocks, or 0, 1, ..), by the CTAs of the cluster (ranks of them). smem: TrxA4Tile::SMEM bytes,
 // 128-byte aligned; what was read of it is ordered before (the caller's barrier).
-template <int HD, bool F32, int R, typename Lim, typename OffQ, typename OffO>
+template <int HD, bool F32, int R, int W, typename Lim, typename OffQ, typename OffO>
 __device__ __forceinline__ void trx_a4_tile(uint8_t *smem, const TrxA4Rows &io, const uint8_t *recs,
                                             const int *list, int n_units, int n_rows, int last, float scale, int ranks,
                                             Lim lim, OffQ off_q, OffO off_o) {
-    constexpr int REC = TrxA4L<HD>::REC, S = TRX_A4_STAGES, W = TRX_A4_WARPS;
+    constexpr int REC = TrxA4L<HD>::REC, S = TRX_A4_STAGES;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = ranks > 1 ? (int)trx_a4_cluster_rank() : 0;
     if (n_units <= W) { // one CTA's work: the others leave, and nobody meets
@@ -933,7 +951,7 @@ __device__ __forceinline__ void trx_a4_tile(uint8_t *smem, const TrxA4Rows &io, 
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads(); // the rings are free
     float *o = reinterpret_cast<float *>(smem), *refs = o + W * R * HD, *sums = refs + W * R;
-    float *co = reinterpret_cast<float *>(smem + TrxA4Tile<HD, R>::PART), *cref = co + R * HD, *csum = cref + R;
+    float *co = reinterpret_cast<float *>(smem + TrxA4Tile<HD, R, W>::PART), *cref = co + R * HD, *csum = cref + R;
     w.store(lane, o + warp * R * HD, refs + warp * R, sums + warp * R);
     __syncthreads();
     constexpr int ITEMS = R * HD / 4;
@@ -962,26 +980,28 @@ __device__ __forceinline__ void trx_a4_tile(uint8_t *smem, const TrxA4Rows &io, 
     }
     if (ranks == 1) return;
     trx_a4_cluster_sync();
-    // the CTAs joined: CTA rank takes an even share of the values, `ranks` neighbouring lanes (a power of two) one of them
-    const int share = ITEMS / ranks, k = tid % ranks;
-    for (int j0 = 0; j0 < share; j0 += 32 * W / ranks) {
-        const int j = j0 + tid / ranks, i = rank * share + min(j, share - 1), r = i / (HD / 4), d = i % (HD / 4) * 4;
-        const float own = trx_a4_peer_load(trx_a4_peer(cref + r, k));
-        float sum = trx_a4_peer_load(trx_a4_peer(csum + r, k));
-        float4 v = trx_a4_peer_load4(trx_a4_peer(co + r * HD + d, k));
+    // the CTAs joined: CTA rank takes an even share of the values, `lanes` neighbouring lanes (a power of two) one of them
+    const int lanes = ranks <= 2 ? 2 : ranks <= 4 ? 4 : ranks <= 8 ? 8 : 16;
+    const int share = (ITEMS + ranks - 1) / ranks, k = tid % lanes, peer = min(k, ranks - 1);
+    for (int j0 = 0; j0 < share; j0 += 32 * W / lanes) {
+        const int j = j0 + tid / lanes, i = min(rank * share + j, ITEMS - 1), r = i / (HD / 4), d = i % (HD / 4) * 4;
+        const float own = trx_a4_peer_load(trx_a4_peer(cref + r, peer));
+        float sum = trx_a4_peer_load(trx_a4_peer(csum + r, peer));
+        float4 v = trx_a4_peer_load4(trx_a4_peer(co + r * HD + d, peer));
         float top = own;
-        for (int x = 1; x < ranks; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        for (int x = 1; x < lanes; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
         const float f = trx_a4_exp2(own - top);
-        sum *= f;
-        v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-        for (int x = 1; x < ranks; x <<= 1) {
+        const bool on = k < ranks; // (a lane without a CTA adds nothing)
+        sum = on ? sum * f : 0.0f;
+        v = on ? make_float4(v.x * f, v.y * f, v.z * f, v.w * f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int x = 1; x < lanes; x <<= 1) {
             sum += __shfl_xor_sync(0xffffffffu, sum, x);
             v.x += __shfl_xor_sync(0xffffffffu, v.x, x);
             v.y += __shfl_xor_sync(0xffffffffu, v.y, x);
             v.z += __shfl_xor_sync(0xffffffffu, v.z, x);
             v.w += __shfl_xor_sync(0xffffffffu, v.w, x);
         }
-        if (k == 0 && j < share && r < n_rows)
+        if (k == 0 && j < share && rank * share + j < ITEMS && r < n_rows)
             trx_a4_out4<F32>(io, off_o(r) + d, make_float4(__fdiv_rn(v.x, sum), __fdiv_rn(v.y, sum),
                                                            __fdiv_rn(v.z, sum), __fdiv_rn(v.w, sum)));
     }
@@ -990,8 +1010,8 @@ __device__ __forceinline__ void trx_a4_tile(uint8_t *smem, const TrxA4Rows &io, 
 
 // The entry a CTA takes in a call of more CTAs than fit at once: the blockIdx.z-th longest, so that the shortest are left
 // for the end (n_entries <= the CTA's threads, all of which call)
-__device__ __forceinline__ int trx_a4_longest(const TrxA4Batch &b, int z) {
-    __shared__ __align__(16) int s_len[32 * TRX_A4_WARPS];
+template <int W> __device__ __forceinline__ int trx_a4_longest(const TrxA4Batch &b, int z) {
+    __shared__ __align__(16) int s_len[32 * W];
     __shared__ int s_entry;
     const int i = threadIdx.x, n = b.n_entries;
     int len = 0;
@@ -1011,13 +1031,13 @@ __device__ __forceinline__ int trx_a4_longest(const TrxA4Batch &b, int z) {
 
 // blockIdx.x = tile of R rows (token-major, a KV head's query heads side by side; the last tiles, whose contexts are the
 // longest, first) x KV head x CTA of the cluster, z the entry
-template <int HD, bool F32, int R>
-__global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
+template <int HD, bool F32, int R, int W>
+__global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
     trx_a4_attend(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int ranks, int sorted) {
     extern __shared__ __align__(128) uint8_t smem[];
     int slot, row0, rows, pos0;
     const int kv = blockIdx.x / ranks % a.n_kv, G = a.n_head / a.n_kv;
-    const int entry = sorted ? trx_a4_longest(b, blockIdx.z) : blockIdx.z;
+    const int entry = sorted ? trx_a4_longest<W>(b, blockIdx.z) : blockIdx.z;
     if (!trx_a4_entry(a, b, entry, slot, row0, rows, pos0)) return;
     const int total = rows * G, tiles = (total + R - 1) / R, tile = tiles - 1 - (int)(blockIdx.x / ranks / a.n_kv);
     if (tile < 0) return;
@@ -1027,7 +1047,7 @@ __global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
         const int x = r0 + r, tok = x / G;
         return (int64_t)(row0 + tok) * stride + (int64_t)(kv * G + x - tok * G) * HD;
     };
-    trx_a4_tile<HD, F32, R>(
+    trx_a4_tile<HD, F32, R, W>(
         smem, io, recs, nullptr, last / TRX_A4_REC + 1, n_rows, last, scale, ranks,
         [&](int r) { return pos0 + (r0 + r) / G; }, [&](int r) { return at(io.q_stride, r); },
         [&](int r) { return at(io.out_stride, r); });
@@ -1051,11 +1071,11 @@ __device__ __forceinline__ uint32_t trx_a4_key(float f) {
 // histograms; each CTA sends its selected blocks to every CTA's list, and the cluster attends to the list.
 // blockIdx.x = (row x tiles of R heads) x CTA of the cluster, y the KV head, z the entry. Dynamic shared memory: the
 // tile's (the keys take its place before it starts), at least keys x 4 bytes, then n_sel ints (list_at).
-template <int HD, bool F32, int R>
-__global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
+template <int HD, bool F32, int R, int W>
+__global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
     trx_a4_select(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int n_sel, int32_t *__restrict__ blocks, int ranks,
                   int list_at) {
-    constexpr int W = TRX_A4_WARPS, N = 32 * W, PW = HD / 64; // words of bounds a lane takes of a block
+    constexpr int N = 32 * W, PW = HD / 64; // words of bounds a lane takes of a block
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int16_t s_pn[2 * HD]; // N, then P, as the bounds
     __shared__ int s_hist[4][256], s_warp[2][W], s_cnt[2], s_pick[2], s_before[2];
@@ -1100,32 +1120,29 @@ __global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < 2 * PW; i++) pn[i] = reinterpret_cast<const int *>(s_pn)[lane * (2 * PW) + i];
         const int8_t *bounds = a.bounds + (at + base) * (2 * HD);
-        for (int g = warp * 8; g < cnt; g += W * 8) { // 8 blocks in flight
-            int w[8][PW], mine = 0;
+        constexpr int F = 16; // blocks in flight
+        for (int g = warp * F; g < cnt; g += W * F) {
+            int w[F][PW], mine = 0;
             float u = 0.0f;
-            if (lane < 8 && g + lane < cnt) u = a.units[at + base + g + lane];
+            if (lane < F && g + lane < cnt) u = a.units[at + base + g + lane];
+            const int8_t *p = bounds + (int64_t)g * (2 * HD) + lane * (4 * PW);
 #pragma unroll
-            for (int i = 0; i < 8; i++)
+            for (int i = 0; i < F; i++) {
+                const bool on = g + i < cnt;
+                if constexpr (PW == 2) {
+                    const int2 v = on ? *reinterpret_cast<const int2 *>(p + i * (2 * HD)) : make_int2(0, 0);
+                    w[i][0] = v.x, w[i][1] = v.y;
+                } else w[i][0] = on ? *reinterpret_cast<const int *>(p + i * (2 * HD)) : 0;
+            }
 #pragma unroll
-                for (int x = 0; x < PW; x++) w[i][x] = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-                if (g + i < cnt) {
-                    const int8_t *p = bounds + (int64_t)(g + i) * (2 * HD) + lane * (4 * PW);
-                    if constexpr (PW == 2) {
-                        const int2 v = *reinterpret_cast<const int2 *>(p);
-                        w[i][0] = v.x, w[i][1] = v.y;
-                    } else w[i][0] = *reinterpret_cast<const int *>(p);
-                }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < F; i++) {
                 int sum = 0;
 #pragma unroll
                 for (int x = 0; x < PW; x++) sum = __dp2a_hi(pn[2 * x + 1], w[i][x], __dp2a_lo(pn[2 * x], w[i][x], sum));
                 sum = __reduce_add_sync(0xffffffffu, sum);
                 if (lane == i) mine = sum;
             }
-            if (lane < 8 && g + lane < cnt) s_key[g + lane] = trx_a4_key(u == INFINITY ? INFINITY : __fmul_rn((float)mine, u));
+            if (lane < F && g + lane < cnt) s_key[g + lane] = trx_a4_key(u == INFINITY ? INFINITY : __fmul_rn((float)mine, u));
         }
         __syncthreads();
         // the largest key that at least n_sel - 1 blocks reach, and how many of the blocks at that key are taken
@@ -1221,7 +1238,7 @@ __global__ void __launch_bounds__(32 * TRX_A4_WARPS, R == 8 ? 2 : 1)
             blocks[((int64_t)(row0 + r) * a.n_kv + kv) * n_sel + i] = i < n_list ? list[i] : -1;
     const uint8_t *recs = a.cache + at * TrxA4L<HD>::BLOCK;
     const int64_t outr = (int64_t)(row0 + r) * io.out_stride + (int64_t)kv * G * HD;
-    trx_a4_tile<HD, F32, R>(
+    trx_a4_tile<HD, F32, R, W>(
         smem, io, recs, list, 2 * (n_list - 1) + (pos % TRX_A4_BLOCK) / TRX_A4_REC + 1, min(R, G - h0), pos, scale,
         ranks, [&](int) { return pos; }, [&](int x) { return qr + (h0 + x) * HD; }, [&](int x) { return outr + (h0 + x) * HD; });
 }
