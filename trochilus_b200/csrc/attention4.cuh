@@ -1078,7 +1078,7 @@ __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
     constexpr int N = 32 * W, PW = HD / 64; // words of bounds a lane takes of a block
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int16_t s_pn[2 * HD]; // N, then P, as the bounds
-    __shared__ int s_hist[4][256], s_warp[2][W], s_cnt[2], s_pick[2], s_before[2];
+    __shared__ int s_hist[4][256], s_warp[2][W], s_cnt[2], s_pick[2][3], s_before[2];
     int slot, row0, rows, pos0;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = blockIdx.y, G = a.n_head / a.n_kv;
     const int tiles = (G + R - 1) / R, r = (int)(blockIdx.x / ranks) / tiles, h0 = (int)(blockIdx.x / ranks) % tiles * R;
@@ -1120,35 +1120,51 @@ __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
 #pragma unroll
         for (int i = 0; i < 2 * PW; i++) pn[i] = reinterpret_cast<const int *>(s_pn)[lane * (2 * PW) + i];
         const int8_t *bounds = a.bounds + (at + base) * (2 * HD);
-        constexpr int F = 16; // blocks in flight
-        for (int g = warp * F; g < cnt; g += W * F) {
-            int w[F][PW], mine = 0;
-            float u = 0.0f;
-            if (lane < F && g + lane < cnt) u = a.units[at + base + g + lane];
+        constexpr int F = 8; // blocks a step; the next step's are on their way
+        int w[2][F][PW];
+        auto look = [&](int (&x)[F][PW], int g) {
             const int8_t *p = bounds + (int64_t)g * (2 * HD) + lane * (4 * PW);
 #pragma unroll
             for (int i = 0; i < F; i++) {
                 const bool on = g + i < cnt;
                 if constexpr (PW == 2) {
                     const int2 v = on ? *reinterpret_cast<const int2 *>(p + i * (2 * HD)) : make_int2(0, 0);
-                    w[i][0] = v.x, w[i][1] = v.y;
-                } else w[i][0] = on ? *reinterpret_cast<const int *>(p + i * (2 * HD)) : 0;
+                    x[i][0] = v.x, x[i][1] = v.y;
+                } else x[i][0] = on ? *reinterpret_cast<const int *>(p + i * (2 * HD)) : 0;
             }
+        };
+        auto score = [&](const int (&x)[F][PW], int g) {
+            int mine = 0;
+            float u = 0.0f;
+            if (lane < F && g + lane < cnt) u = a.units[at + base + g + lane];
 #pragma unroll
             for (int i = 0; i < F; i++) {
                 int sum = 0;
 #pragma unroll
-                for (int x = 0; x < PW; x++) sum = __dp2a_hi(pn[2 * x + 1], w[i][x], __dp2a_lo(pn[2 * x], w[i][x], sum));
+                for (int k = 0; k < PW; k++) sum = __dp2a_hi(pn[2 * k + 1], x[i][k], __dp2a_lo(pn[2 * k], x[i][k], sum));
                 sum = __reduce_add_sync(0xffffffffu, sum);
                 if (lane == i) mine = sum;
             }
             if (lane < F && g + lane < cnt) s_key[g + lane] = trx_a4_key(u == INFINITY ? INFINITY : __fmul_rn((float)mine, u));
+        };
+        look(w[0], warp * F);
+#pragma unroll 1
+        for (int g = warp * F; g < cnt; g += 2 * W * F) {
+            look(w[1], g + W * F);
+            score(w[0], g);
+            look(w[0], g + 2 * W * F);
+            score(w[1], g + W * F);
         }
         __syncthreads();
         // the largest key that at least n_sel - 1 blocks reach, and how many of the blocks at that key are taken
         uint32_t key = 0;
         int want = n_sel - 1;
-        for (int pass = 0; pass < 4; pass++) {
+        auto meet = [&] {
+            if (ranks > 1) trx_a4_cluster_sync();
+            else __syncthreads();
+        };
+        bool all = false; // the last bin's blocks are all taken: the key's other bits do not matter
+        for (int pass = 0; pass < 4 && !all; pass++) {
             const int shift = 24 - 8 * pass;
             const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + 8);
             for (int i0 = 0; i0 < cnt; i0 += N) {
@@ -1158,9 +1174,10 @@ __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
                 const uint32_t same = __match_any_sync(0xffffffffu, bin); // (most keys share their first bits)
                 if (on && lane == __ffs(same) - 1) atomicAdd(&s_hist[pass][bin], __popc(same));
             }
-            trx_a4_cluster_sync();
+            meet();
             int n = 0; // thread: a bin (of 256)
-            if (tid < 256)
+            if (ranks == 1) n = s_hist[pass][tid];
+            else
                 for (int k = 0; k < ranks; k++) n += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_hist[pass][tid], k)));
             int above = n; // its blocks and those of the higher bins
             for (int s = 1; s < 32; s <<= 1) {
@@ -1170,35 +1187,39 @@ __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
             if (lane == 0) s_warp[0][warp] = above;
             __syncthreads();
             for (int i = warp + 1; i < W; i++) above += s_warp[0][i];
-            if (above >= want && above - n < want) s_pick[0] = tid, s_pick[1] = want - (above - n);
+            if (above >= want && above - n < want) s_pick[pass & 1][0] = tid, s_pick[pass & 1][1] = want - (above - n), s_pick[pass & 1][2] = n;
             __syncthreads();
-            key |= (uint32_t)s_pick[0] << shift;
-            want = s_pick[1];
-            __syncthreads();
+            key |= (uint32_t)s_pick[pass & 1][0] << shift;
+            want = s_pick[pass & 1][1];
+            all = want == s_pick[pass & 1][2] && key > 0;
         }
+        if (all) key--, want = 0;
         // this CTA's blocks above the key and at it, and those of the CTAs before
-        int above = 0, equal = 0;
-        for (int i = tid; i < cnt; i += N) above += s_key[i] > key, equal += s_key[i] == key;
-        above = __reduce_add_sync(0xffffffffu, above);
-        equal = __reduce_add_sync(0xffffffffu, equal);
-        if (lane == 0) s_warp[0][warp] = above, s_warp[1][warp] = equal;
-        __syncthreads();
-        if (tid < 2) {
-            int n = 0;
-            for (int i = 0; i < W; i++) n += s_warp[tid][i];
-            s_cnt[tid] = n;
-        }
-        trx_a4_cluster_sync();
-        if (tid == 0) {
-            int eq = 0, n = 0;
-            for (int k = 0; k < rank; k++) {
-                n += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_cnt[0], k)));
-                eq += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_cnt[1], k)));
+        int place = 0, ties = 0;
+        if (ranks > 1) {
+            int above = 0, equal = 0;
+            for (int i = tid; i < cnt; i += N) above += s_key[i] > key, equal += s_key[i] == key;
+            above = __reduce_add_sync(0xffffffffu, above);
+            equal = __reduce_add_sync(0xffffffffu, equal);
+            if (lane == 0) s_warp[0][warp] = above, s_warp[1][warp] = equal;
+            __syncthreads();
+            if (tid < 2) {
+                int n = 0;
+                for (int i = 0; i < W; i++) n += s_warp[tid][i];
+                s_cnt[tid] = n;
             }
-            s_before[0] = n + min(eq, want), s_before[1] = eq;
+            trx_a4_cluster_sync();
+            if (tid == 0) {
+                int eq = 0, n = 0;
+                for (int k = 0; k < rank; k++) {
+                    n += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_cnt[0], k)));
+                    eq += __float_as_int(trx_a4_peer_load(trx_a4_peer(&s_cnt[1], k)));
+                }
+                s_before[0] = n + min(eq, want), s_before[1] = eq;
+            }
+            __syncthreads();
+            place = s_before[0], ties = s_before[1];
         }
-        __syncthreads();
-        int place = s_before[0], ties = s_before[1];
         for (int i0 = 0; i0 < cnt; i0 += N) { // ascending
             const int i = i0 + tid;
             const bool eq = i < cnt && s_key[i] == key;
@@ -1222,13 +1243,15 @@ __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
             ties = all;
             if (take) {
                 to += __popc(t & ((1u << lane) - 1));
-                for (int k = 0; k < ranks; k++)
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(trx_a4_peer(list + to, k)), "r"(base + i) : "memory");
+                if (ranks == 1) list[to] = i;
+                else
+                    for (int k = 0; k < ranks; k++)
+                        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(trx_a4_peer(list + to, k)), "r"(base + i) : "memory");
             }
             __syncthreads();
         }
         if (tid == 0) list[n_sel - 1] = home;
-        trx_a4_cluster_sync();
+        meet();
     } else {
         for (int i = tid; i < n_list; i += N) list[i] = n_sel == 1 ? home : i;
     }
