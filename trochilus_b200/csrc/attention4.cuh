@@ -118,7 +118,7 @@ template <typename T> __device__ __forceinline__ void trx_a4_store8(T *p, const 
                                                trx_a4_pack2(x[4], x[5], p), trx_a4_pack2(x[6], x[7], p));
 }
 
-// three-operand minimum and maximum (a NaN beside a number is dropped)
+// three-operand minimum and maximum (a NaN beside a number is dropped; _nan: stays)
 __device__ __forceinline__ float trx_a4_min3(float a, float b, float c) {
     float d;
     asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -129,15 +129,23 @@ __device__ __forceinline__ float trx_a4_max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ float trx_a4_max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
-// codes with those whose quotient is next to a border taken exactly (seldom called, and kept out of the loops)
+// codes with those whose quotient is within `near` of a border (or of what 32 bits tell apart from one) taken exactly
+// (seldom called, and kept out of the loops): x is compared with the border m + (k + 1/2) d itself, whose second term is
+// exact: with its nearest float s, and where x is s, with what s dropped
 __device__ __noinline__ uint32_t trx_a4_near(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float m,
-                                             float d, float rd, uint32_t codes) {
+                                             float d, float rd, float near, uint32_t codes) {
     const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float u = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)) * 15.0f, k = floorf(u);
-        if (fabsf(__fsub_rn(__fsub_rn(u, k), 0.5f)) > 3.0e-5f) continue;
+        const float u = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)) * 15.0f;
+        float k = floorf(u);
+        if (fabsf(__fsub_rn(__fsub_rn(u, k), 0.5f)) > 2.0f * near) continue;
         const float h = __fmul_rn(__fadd_rn(k, 0.5f), d), s = __fadd_rn(m, h);
         const float t = __fsub_rn(s, m); // s + lost = m + h
         const float lost = __fadd_rn(__fsub_rn(m, __fsub_rn(s, t)), __fsub_rn(h, t));
@@ -148,24 +156,21 @@ __device__ __noinline__ uint32_t trx_a4_near(float x0, float x1, float x2, float
 }
 
 // The 8 codes (4 bits each, value j at bits 4 j), scale and minimum of 8 values of a group whose other 24 lie in the
-// lanes next to this one (4 aligned lanes a group; the whole warp calls); x becomes what they stand for.
+// lanes next to this one (4 aligned lanes a group; the whole warp calls). VALUES: x becomes what they stand for.
 // Both are taken in 32 bits, and exactly where that may round to another side. (hi - m) / 15 is off by less than 2^-22 of
 // itself, so it is certain unless 1 - 2^-21 and 1 + 2^-21 times it round apart (then: in 64 bits). A quotient, kept within
-// 0 .. 15 as 15 times the saturated (x - m) / (15 d) (15 d is exact), is off by less than 4 x 2^-24 x 15 < 4e-6, so it is
-// certain unless it is within 2e-5 of a border. Then x is compared with the border m + (k + 1/2) d itself, whose second
-// term is exact: with its nearest float s, and where x is s, with what s dropped. (16-bit inputs meet such borders often.)
-__device__ __forceinline__ uint32_t trx_a4_quant(float (&x)[8], uint16_t &d16, uint16_t &m16) {
-    float lo = trx_a4_min3(x[0], x[1], x[2]), hi = trx_a4_max3(x[0], x[1], x[2]), none = 0.0f;
-    lo = trx_a4_min3(lo, x[3], x[4]), hi = trx_a4_max3(hi, x[3], x[4]);
-    lo = trx_a4_min3(lo, x[5], x[6]), hi = trx_a4_max3(hi, x[5], x[6]);
-    lo = fminf(lo, x[7]), hi = fmaxf(hi, x[7]);
-#pragma unroll
-    for (int j = 0; j < 8; j++) none = __fmaf_rn(x[j], 0.0f, none); // (0, or NaN where a value is not finite)
+// 0 .. 15, is 15 times the saturated x r - m r, r = 1 / (15 d) (15 d is exact): off by less than 4 x 2^-24 x 15 < 4e-6
+// where m r is small, and by the rounding of m r, 15 x 2^-24 |m r|, where it is not: it is certain unless it is within
+// near = 1e-5 + 2^-19 |m r| of a border. (16-bit inputs meet borders often.)
+template <bool VALUES> __device__ __forceinline__ uint32_t trx_a4_quant(float (&x)[8], uint16_t &d16, uint16_t &m16) {
+    float lo = trx_a4_min3(x[0], x[1], x[2]), hi = trx_a4_max3_nan(x[0], x[1], x[2]);
+    lo = trx_a4_min3(lo, x[3], x[4]), hi = trx_a4_max3_nan(hi, x[3], x[4]);
+    lo = trx_a4_min3(lo, x[5], x[6]), hi = trx_a4_max3_nan(hi, x[5], x[6]);
+    lo = fminf(lo, x[7]), hi = trx_a4_max3_nan(hi, hi, x[7]);
 #pragma unroll
     for (int s = 1; s <= 2; s <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-        none += __shfl_xor_sync(0xffffffffu, none, s);
+        hi = trx_a4_max3_nan(hi, hi, __shfl_xor_sync(0xffffffffu, hi, s));
     }
     const __half mh = __float2half_rn(lo);
     const float m = __half2float(mh);
@@ -174,32 +179,37 @@ __device__ __forceinline__ uint32_t trx_a4_quant(float (&x)[8], uint16_t &d16, u
     if (__half_as_ushort(dh) != __half_as_ushort(__float2half_rn(__fmul_rn(step, 1.0f + 4.76837158e-7f))))
         dh = __double2half(__ddiv_rn(fmax(__dsub_rn((double)hi, (double)m), 0.0), 15.0));
     const float d = __half2float(dh);
-    const bool bad = none != 0.0f || !(fabsf(m) <= 65504.0f) || !(d <= 65504.0f);
+    // (an infinity among the values makes m or d one; a NaN leaves hi one)
+    const bool bad = hi != hi || !(fabsf(m) <= 65504.0f) || !(d <= 65504.0f);
     d16 = bad ? (uint16_t)0x7fff : __half_as_ushort(dh);
     m16 = bad ? (uint16_t)0 : __half_as_ushort(mh);
     if (bad || d == 0.0f) {
+        if constexpr (VALUES)
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = bad ? __int_as_float(0x7fffffff) : m;
+            for (int j = 0; j < 8; j++) x[j] = bad ? __int_as_float(0x7fffffff) : m;
         return 0;
     }
-    const float rd = __frcp_rn(__fmul_rn(15.0f, d));
-    uint32_t codes = 0;
+    const float r = __frcp_rn(__fmul_rn(15.0f, d)), mr = __fmul_rn(m, -r), near = __fmaf_rn(fabsf(mr), 1.9073486e-6f, 1.0e-5f);
     float q[8], far[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) { // (an integer's nearest: the low bits of 1.5 x 2^23 + 15 v)
-        const float v = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)), t = __fmaf_rn(v, 15.0f, 12582912.0f);
-        q[j] = __fsub_rn(t, 12582912.0f);
+    for (int j = 0; j < 8; j++) { // (an integer's nearest: what 1.5 x 2^23 + 15 v keeps)
+        const float v = __saturatef(__fmaf_rn(x[j], r, mr));
+        q[j] = __fsub_rn(__fmaf_rn(v, 15.0f, 12582912.0f), 12582912.0f);
         far[j] = fabsf(__fmaf_rn(v, 15.0f, -q[j]));
-        codes += __float_as_uint(t) * (1u << (4 * j));
     }
-    codes -= 0x3f400000u; // (the sum of the constants that went in with the codes)
-    if (fmaxf(trx_a4_max3(trx_a4_max3(far[0], far[1], far[2]), far[3], far[4]), trx_a4_max3(far[5], far[6], far[7])) > 0.49998f) {
-        codes = trx_a4_near(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], m, d, rd, codes);
+    // four codes are a number below 2^16, whose bits 8388608 + it holds
+    const float c0 = __fmaf_rn(q[3], 4096.0f, __fmaf_rn(q[2], 256.0f, __fmaf_rn(q[1], 16.0f, q[0])));
+    const float c1 = __fmaf_rn(q[7], 4096.0f, __fmaf_rn(q[6], 256.0f, __fmaf_rn(q[5], 16.0f, q[4])));
+    uint32_t codes = __byte_perm(__float_as_uint(__fadd_rn(c0, 8388608.0f)), __float_as_uint(__fadd_rn(c1, 8388608.0f)), 0x5410);
+    if (fmaxf(trx_a4_max3(trx_a4_max3(far[0], far[1], far[2]), far[3], far[4]), trx_a4_max3(far[5], far[6], far[7])) > 0.5f - near) {
+        codes = trx_a4_near(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], m, d, r, near, codes);
+        if constexpr (VALUES)
 #pragma unroll
-        for (int j = 0; j < 8; j++) q[j] = (float)((codes >> (4 * j)) & 15);
+            for (int j = 0; j < 8; j++) q[j] = (float)((codes >> (4 * j)) & 15);
     }
+    if constexpr (VALUES)
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = __fmaf_rn(d, q[j], m); // (d x code is exact)
+        for (int j = 0; j < 8; j++) x[j] = __fmaf_rn(d, q[j], m); // (d x code is exact)
     return codes;
 }
 
@@ -302,7 +312,7 @@ __global__ void __launch_bounds__(256, 3) trx_a4_write(TrxA4 a, TrxA4Batch b, co
         for (int r = 0; r < 2; r++) {
             trx_a4_floats(rk[r], x[r]);
             if (__any_sync(0xffffffffu, on[r])) {
-                const uint32_t c = trx_a4_quant(x[r], d, m);
+                const uint32_t c = trx_a4_quant<true>(x[r], d, m);
                 if (on[r]) {
                     *reinterpret_cast<uint32_t *>(s_rec + trx_a4_kcode<HD>(p[r], l)) = c;
                     if ((l & 3) == 0) {
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(256, 3) trx_a4_write(TrxA4 a, TrxA4Batch b, co
         for (int r = 0; r < 2; r++)
             if (__any_sync(0xffffffffu, on[r])) {
                 trx_a4_floats(rv[r], x[r]);
-                const uint32_t c = trx_a4_quant(x[r], d, m);
+                const uint32_t c = trx_a4_quant<false>(x[r], d, m);
                 if (on[r]) {
                     *reinterpret_cast<uint16_t *>(s_rec + trx_a4_vcode<HD>(p[r], l, 0)) = (uint16_t)c;
                     *reinterpret_cast<uint16_t *>(s_rec + trx_a4_vcode<HD>(p[r], l, 1)) = (uint16_t)(c >> 16);
