@@ -313,7 +313,7 @@ TRMOE_API int tr_gpu_attn_warm(tr_gpu_attn *a, uint64_t ns);
  * none writes what another one of them reads or writes (the caller orders those). Each makes the session's device
  * current on the calling thread; every pointer is memory of that device, rows of `type` (TRMOE_F32, TRMOE_F16 or
  * TRMOE_BF16), a row's heads side by side, strides in values between rows; rows start on 16-byte boundaries (the
- * stride too) and must not overlap in an output. 0, or -1 with trmoe_last_error(). */
+ * stride too); an output's rows overlap neither each other nor an input. 0, or -1 with trmoe_last_error(). */
 typedef struct tr_gpu_attn4 tr_gpu_attn4;
 #define TRMOE_ATTN4_BLOCK 64      /* positions of a selectable block */
 #define TRMOE_ATTN4_MAX_GROUP 256 /* query heads a KV head */
@@ -359,8 +359,11 @@ TRMOE_API int tr_gpu_attn4_write_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gp
 TRMOE_API int tr_gpu_attn4_read_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type, void *k,
                                     int64_t k_stride, void *v, int64_t v_stride, void *stream);
 /* out row = softmax(scale q.k) v over positions 0 .. p of the row's sequence, p the row's own position (whose key and
- * value a write has stored before): one row an entry is a decode step, several are a prompt or drafted tokens. q and
- * out [n_tok][n_head * head_dim]. Scores, softmax and sums are in 32 bits. */
+ * value a write has stored before, as all positions before it): one row an entry is a decode step, several are a prompt
+ * or drafted tokens. q and out [n_tok][n_head * head_dim]. Scores and sums are in 32 bits, and so is the rest for f32
+ * rows (two 16-bit parts of each factor); for 16-bit rows a probability is rounded to f16 (2^-12 relative), and in calls
+ * of many rows the keys and values are. A NaN or an infinity among the positions that a row sees makes that head's
+ * output, or its group of 32 values, NaN; among others it does not matter. */
 TRMOE_API int tr_gpu_attn4_attend_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type,
                                       const void *q, int64_t q_stride, float scale, void *out, int64_t out_stride,
                                       void *stream);

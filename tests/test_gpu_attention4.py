@@ -262,6 +262,22 @@ def test_nan_and_infinity(cuda, kind):
     s.close()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_scales_and_query_sizes(cuda, kind):
+    """a scale of 0, negative ones, queries that are zero, tiny and large"""
+    rng = np.random.default_rng(18)
+    s = Session(cuda, 1, 4, 2, 64, 500)
+    s.write([(0, 0, 500)], *_rows(rng, 500, 2, 64), kind)
+    q = rng.normal(size=(5, 4, 64)).astype(np.float32)
+    q[1] = 0
+    q[2] *= 1e-7 if kind == "f16" else 1e-30
+    q[3] *= 50
+    for scale in (0.0, -0.2, 0.05, 1e-6, 3.0):
+        s.check_attend([(0, 499, 1), (0, 100, 1), (0, 3, 1), (0, 64, 1), (0, 0, 1)], q, kind, scale=scale)
+        s.check_attend([(0, 430, 5)], q, kind, scale=scale, n_sel=3)
+    s.close()
+
+
 def test_large_scores_and_a_far_sink(cuda):
     """scores hundreds apart; one position with nearly all the weight and tiny values beside a thousand others"""
     rng = np.random.default_rng(6)

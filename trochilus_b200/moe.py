@@ -6,6 +6,8 @@ kernels would. It raises when the library is missing: there is no fallback of an
   GpuMoe          the layer hook (tr_gpu_moe_*): Trochilus's forward_layer MoE block
                   (src/models/olmoe.c:1845-1933) on the GPU, weights resident in HBM
   matmul_grouped  tr_matmul_grouped (src/kernels/kernels.h:244-245) on host arrays
+  GpuAttn         the decode attention session (tr_gpu_attn_*, src/backend/gpu_attn.h)
+  GpuAttn4        attention over a KV cache in 4 bits (tr_gpu_attn4_*), device rows
   matmul, softmax, swiglu   tr_matmul, tr_softmax, tr_swiglu
   q4x_road, q4x_prepare, matmul_q4x_prepared, swiglu_prepare   Q4_K's prepared road (kernels.h:280-300, 350)
 """
