@@ -281,16 +281,15 @@ __global__ void __launch_bounds__(256, 3) trx_a4_write(TrxA4 a, TrxA4Batch b, co
     uint8_t *rec = a.cache + at * Y::BLOCK;
     const int p0 = max(pos0, first) - first, p1 = min(pos0 + rows - first, TRX_A4_BLOCK);
     const int l = tid % L, g = l >> 2;
-    int same = 0;
-    for (int j = tid; j < e; j += 256) same |= b.slot[j] == slot;
+    for (int j = 0; j < e; j += 32) // (each warp looks for itself: no barrier before the rows)
+        if (__any_sync(0xffffffffu, j + (tid & 31) < e && b.slot[j + (tid & 31)] == slot)) {
+            if (tid == 0) atomicCAS(a.err, 0, TRX_A4_SAME_SLOT);
+            return;
+        }
     float lo[8], hi[8];
     int bad = 0;
 #pragma unroll
     for (int j = 0; j < 8; j++) lo[j] = INFINITY, hi[j] = -INFINITY;
-    if (__syncthreads_or(same)) {
-        if (tid == 0) atomicCAS(a.err, 0, TRX_A4_SAME_SLOT);
-        return;
-    }
 #pragma unroll 1
     for (int i = 0; i < N; i += 2) { // two rows a lane
         int p[2];

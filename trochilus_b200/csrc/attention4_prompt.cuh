@@ -10,7 +10,7 @@
 //                stores as rows, dim 32 g + 4 n + i in row 32 g + 8 i + n (O's columns are put right at the end)
 //   warp 15      one thread issues tcgen05.mma (kind::f16, f32 accumulators in tensor memory): S = Q K^T and O += P V, the
 //                tiles in turn, so that one's products run under the other's softmax
-//   warps 0-7    a thread a row, 32 scores at a time: 2^(s - ref) as f16 back into tensor memory (P takes S's place) and
+//   warps 0-7    a thread a row, 64 scores at a time: 2^(s - ref) as f16 back into tensor memory (P takes S's place) and
 //                their sum, against the reference of the scores before; where one passes it by 2^8, the references of
 //                the warp's rows move up and O, P and the sums so far are rescaled (p stays below 2^15)
 // The loops are kept short: with all of them unrolled the warps waited for instructions (2 x 2048 rows of 32 heads at 4096
@@ -266,14 +266,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                     }
                     return trx_a4_max3(fmaxf(best[0], best[1]), best[2], best[3]) * c;
                 };
-                auto take = [&](uint32_t(&r)[32], float best, int at) {
-                    if (__any_sync(0xffffffffu, best > top + 8.0f)) { // (S j is complete: so are O's products before it)
-                        top = fmaxf(top, best);
-                        const float next = top == -1.0e30f ? -1.0e30f : top - 7.0f, f = ref == next ? 1.0f : trx_a4_exp2(ref - next);
-                        ref = next;
-                        sum = trx_mul2(sum, trx_pack2(f, f));
-                        trx_a4p_rescale(to, j > 0 ? HD : 0, ts, at / 2, f);
-                    }
+                auto take = [&](uint32_t(&r)[32], int at) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
@@ -282,21 +275,25 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                         p[i / 2] = trx_a4_half2(x, y);
                         asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(trx_pack2(x, y)));
                     }
-                    trx_a4p_st16(ts + at / 2, p); // (S's columns at / 2 .. have been read)
+                    trx_a4p_st16(ts + at / 2, p);
                 };
-                uint32_t r0[32], r1[32];
-                trx_tmem_ld32_nw(ts, r0);
-                trx_a4p_landed(r0);
 #pragma unroll 1
-                for (int h = 0; h < 128; h += 64) { // (the next 32 are on their way while 32 are taken)
+                for (int h = 0; h < 128; h += 64) {
+                    uint32_t r0[32], r1[32];
+                    trx_tmem_ld32_nw(ts + h, r0);
                     trx_tmem_ld32_nw(ts + h + 32, r1);
-                    float best = look(r0, h);
-                    take(r0, best, h);
-                    trx_a4p_landed(r1);
-                    if (h == 0) trx_tmem_ld32_nw(ts + 64, r0);
-                    best = look(r1, h + 32);
-                    take(r1, best, h + 32);
                     trx_a4p_landed(r0);
+                    trx_a4p_landed(r1);
+                    const float best = fmaxf(look(r0, h), look(r1, h + 32));
+                    if (__any_sync(0xffffffffu, best > top + 8.0f)) { // (S j is complete: so are O's products before it)
+                        top = fmaxf(top, best);
+                        const float next = top == -1.0e30f ? -1.0e30f : top - 7.0f, f = ref == next ? 1.0f : trx_a4_exp2(ref - next);
+                        ref = next;
+                        sum = trx_mul2(sum, trx_pack2(f, f));
+                        trx_a4p_rescale(to, j > 0 ? HD : 0, ts, h / 2, f);
+                    }
+                    take(r0, h);
+                    take(r1, h + 32); // (S's columns h / 2 .. h / 2 + 31 have been read)
                 }
                 trx_tmem_wait_st();
                 trx_tc_fence_before();
