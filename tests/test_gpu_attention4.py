@@ -522,6 +522,24 @@ def test_long_contexts(cuda, kind, heads, kv, hd):
     s.close()
 
 
+def test_f32_sums_over_long_contexts(cuda):
+    """f32 rows: the error must not grow with the number of positions. Counted against the outputs' norm, for values of mean 0
+    whose sum is as large as their roundings' sums let it be: a probability in two f16 parts and its product with a scale
+    2^-21, the exponential 2^-22, a score near 0 of query values in two parts 2^-20, a value's minimum 2^-21, 60 rounded
+    additions a warp 2^-24 x 8, its sums' and the joins' 2^-23: below 2^-18.5 together were all at their worst, and they
+    are independent, so that a norm over 1024 outputs stays below 2^-19."""
+    rng = np.random.default_rng(23)
+    ctx = 100_000
+    s = Session(cuda, 1, 8, 8, 128, ctx)
+    s.write([(0, 0, ctx)], *[rng.normal(size=(ctx, 8, 128)).astype(np.float32) for _ in "kv"])
+    q = rng.normal(size=(1, 8, 128)).astype(np.float32)
+    got = s.attend([(0, ctx - 1, 1)], q)[0]
+    want, _ = orc.attention(q[0], s.k[0], s.v[0], 128 ** -0.5, None)
+    assert np.linalg.norm(got - want) < 2 ** -19 * np.linalg.norm(want)
+    s.s.check()
+    s.close()
+
+
 def test_overlapping_calls(cuda):
     """one session's calls on two streams at once, eager and as two captured graphs: each gives what it gives alone"""
     torch = cuda

@@ -264,6 +264,8 @@ template <int HD> __device__ __forceinline__ void trx_a4_value8(const uint8_t *r
 // count too; such a block is no earlier one of any query, so that its bounds are not read.
 // The records are put together in shared memory (a row's value codes lie 2 bytes here and there) and leave it 16 bytes a
 // thread where the block is written whole, else as the rows' own pieces.
+// What bounds it: the quantiser's instructions. 4096 rows of 16 heads of 128 (f32, 77 MB): 22 us, 0.54 of the measured copy
+// rate. Keys and values in CTAs of their own: 31 us against 29 then.
 template <int HD, typename T>
 __global__ void __launch_bounds__(256, 3) trx_a4_write(TrxA4 a, TrxA4Batch b, const T *__restrict__ k, int64_t k_stride,
                                                     const T *__restrict__ v, int64_t v_stride) {
@@ -397,7 +399,8 @@ __global__ void __launch_bounds__(256, 3) trx_a4_write(TrxA4 a, TrxA4Batch b, co
 }
 
 // The rows of an entry's block read back (the write's grid), by way of shared memory; a lane 16 bytes of a row, so that a
-// warp writes 512 contiguous bytes (f32 rows by 32 bytes a lane: 20.5 us for 4096 rows of 16 heads of 128)
+// warp writes 512 contiguous bytes. Bound by HBM: 4096 rows of 16 heads of 128 (f32, 77 MB) 11.6 us, the measured copy rate
+// (by 32 bytes a lane 20.5 us).
 template <int HD, typename T>
 __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__restrict__ k, int64_t k_stride,
                                                    T *__restrict__ v, int64_t v_stride) {
@@ -453,7 +456,10 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 //            first); a group is two of them, then d; the minima's sums are one m16n8k8 with B = sum_i x_gi in two f16
 //            parts
 //   softmax  a reference a row, which moves only when a score passes it (16-bit rows: by 2^8), so that the usual record
-//            needs one vote and no reduction; p in f16 (f32 rows: two f16 parts, 22 bits), transposed in registers (movmatrix)
+//            needs one vote and no reduction; p in f16 (f32 rows: two f16 parts, 22 bits), transposed in registers (movmatrix).
+//            16-bit rows' p, p d and subnormal codes leave f16 outputs 6e-4 off 64 bits at 100,000 positions of random values,
+//            whose outputs' own rounding is 2e-4 (bf16: 1.7e-3, all of it the outputs'); codes as integers 3.4e-4, for a third
+//            more time
 //   outputs  mma m16n8k16: A = 16 dims x 16 positions of codes, B = p_t d_tg of 8 rows; one more with the minima (and
 //            ones, which sum p) as A.
 // 16 query rows of f16 or bf16 type, or 8 (R), share the codes' unpacking; scores, sums and outputs are f32.
@@ -463,6 +469,10 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 // A cluster of CTAs shares one tile of query rows: its warps take records in turn, their results are joined in each
 // CTA through shared memory, and the CTAs' through distributed shared memory, so that no workspace or second launch is
 // needed and overlapping calls share nothing.
+//
+// What bounds it: HBM where the CTAs fill the GPU (64 sequences of 8192 positions, 32 heads over 8 of 128, bf16: 117 us, 5.7
+// TB/s, 0.87 of the measured copy rate); a record's 449 warp instructions where clusters leave SMs idle (one such sequence of
+// 131,072 positions: 46.7 us, 3.6 TB/s on 80 SMs) or many rows share the records (f32 prompts).
 #define TRX_A4_STAGES 2
 
 __device__ __forceinline__ void trx_a4_mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -604,6 +614,15 @@ template <bool EXACT, int MID = 0> __device__ __forceinline__ void trx_a4_codes(
     trx_a4_half_codes<EXACT, MID>(w, a);
     trx_a4_half_codes<EXACT, MID>(w >> 8, b);
     h[0] = a[0], h[1] = a[1], h[2] = b[0], h[3] = b[1];
+}
+
+__device__ __forceinline__ void trx_a4_add4(float (&a)[4], const float (&b)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        trx_f2 x = trx_pack2(a[i], a[i + 1]);
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(trx_pack2(b[i], b[i + 1])));
+        a[i] = trx_lo(x), a[i + 1] = trx_hi(x);
+    }
 }
 
 // One warp's state for R query rows: NT tiles of 8
@@ -874,8 +893,11 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
             }
 #pragma unroll
             for (int r = 0; r < NT; r++) {
-                trx_a4_mma16(accm[r], m[0], ml[0], m[1], ml[1], p[0][r], p[1][r]);
-                if constexpr (F32) trx_a4_mma16(accm[r], m[0], ml[0], m[1], ml[1], pl[0], pl[1]);
+                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float(&o)[4] = F32 ? y : accm[r];
+                if constexpr (F32) trx_a4_mma16(o, m[0], ml[0], m[1], ml[1], pl[0], pl[1]);
+                trx_a4_mma16(o, m[0], ml[0], m[1], ml[1], p[0][r], p[1][r]);
+                if constexpr (F32) trx_a4_add4(accm[r], y);
             }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
@@ -885,16 +907,22 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
                     uint32_t b0 = trx_a4_hmul2(p[0][r], d[0][g]), b1 = trx_a4_hmul2(p[1][r], d[1][g]);
+                    // (f32: 16 positions from 0, then added with rounding: the tensor core's additions to a sum do not round,
+                    // and 131,072 positions of 8 KV heads were 7.6e-6 off 64 bits, now 8.6e-7, for 6 to 8 % of the time.
+                    // 16-bit rows: no change beside their roundings of p)
+                    float y[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                    float(&o0)[4] = F32 ? y[0] : acc[g][0][r], (&o1)[4] = F32 ? y[1] : acc[g][1][r];
                     if constexpr (F32) { // p d in two parts: what the product's rounding drops, and the lower part's product
                         uint32_t l0 = trx_a4_hfma2(pl[0], d[0][g], trx_a4_hfms2(p[0][r], d[0][g], b0));
                         uint32_t l1 = trx_a4_hfma2(pl[1], d[1][g], trx_a4_hfms2(p[1][r], d[1][g], b1));
                         if constexpr (MASK) l0 &= ok[0][r], l1 &= ok[1][r];
-                        trx_a4_mma16(acc[g][0][r], u[0], u[1], v[0], v[1], l0, l1);
-                        trx_a4_mma16(acc[g][1][r], u[2], u[3], v[2], v[3], l0, l1);
+                        trx_a4_mma16(o0, u[0], u[1], v[0], v[1], l0, l1);
+                        trx_a4_mma16(o1, u[2], u[3], v[2], v[3], l0, l1);
                     }
                     if constexpr (MASK) b0 &= ok[0][r], b1 &= ok[1][r];
-                    trx_a4_mma16(acc[g][0][r], u[0], u[1], v[0], v[1], b0, b1);
-                    trx_a4_mma16(acc[g][1][r], u[2], u[3], v[2], v[3], b0, b1);
+                    trx_a4_mma16(o0, u[0], u[1], v[0], v[1], b0, b1);
+                    trx_a4_mma16(o1, u[2], u[3], v[2], v[3], b0, b1);
+                    if constexpr (F32) trx_a4_add4(acc[g][0][r], y[0]), trx_a4_add4(acc[g][1][r], y[1]);
                 }
             }
         }
@@ -1095,6 +1123,9 @@ __device__ __forceinline__ uint32_t trx_a4_key(float f) {
 // histograms; each CTA sends its selected blocks to every CTA's list, and the cluster attends to the list.
 // blockIdx.x = (row x tiles of R heads) x CTA of the cluster, y the KV head, z the entry. Dynamic shared memory: the
 // tile's (the keys take its place before it starts), at least keys x 4 bytes, then n_sel ints (list_at).
+// What bounds it: latency. 24 x 4 rows, 16 of up to 512 blocks, 16 heads of 64 over 4, f32: 35 us in 1.3 rounds of CTAs, of
+// whose 34,500 cycles 10 % load the queries, 24 % score, 16 % find the threshold, 5 % make the list, 45 % attend. One row,
+// 32 of 2047 blocks, 32 heads over 8 of 128, bf16: 17 us (all positions 47).
 template <int HD, bool F32, int R, int W>
 __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
     trx_a4_select(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int n_sel, int32_t *__restrict__ blocks, int ranks,
