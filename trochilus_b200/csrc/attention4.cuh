@@ -137,14 +137,15 @@ __device__ __forceinline__ float trx_a4_max3_nan(float a, float b, float c) {
 
 // codes with those whose quotient is within `near` of a border (or of what 32 bits tell apart from one) taken exactly
 // (seldom called, and kept out of the loops): x is compared with the border m + (k + 1/2) d itself, whose second term is
-// exact: with its nearest float s, and where x is s, with what s dropped
+// exact: with its nearest float s, and where x is s, with what s dropped. (The last border is 14.5 d: a scale rounded down
+// among f16's smallest numbers leaves quotients up to 22, and codes stay 15.)
 __device__ __noinline__ uint32_t trx_a4_near(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7, float m,
                                              float d, float rd, float near, uint32_t codes) {
     const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float u = __saturatef(__fmul_rn(__fsub_rn(x[j], m), rd)) * 15.0f;
-        float k = floorf(u);
+        const float k = fminf(floorf(u), 14.0f);
         if (fabsf(__fsub_rn(__fsub_rn(u, k), 0.5f)) > 2.0f * near) continue;
         const float h = __fmul_rn(__fadd_rn(k, 0.5f), d), s = __fadd_rn(m, h);
         const float t = __fsub_rn(s, m); // s + lost = m + h
