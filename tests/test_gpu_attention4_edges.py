@@ -3,9 +3,30 @@ barely, against definitions in 64 bits with bounds for each value (tests/attn4_b
 import numpy as np
 import pytest
 
-from tests.test_gpu_attention4 import Session
+from tests import attn4_bounds as bnd
+from tests import attn4_oracle as orc
+from tests.test_gpu_attention4 import Session, _rows
 
 pytestmark = pytest.mark.gpu
+
+
+def _check(s, entries, q, kind, scale=None, n_sel=None, prompt=False):
+    """attend (or select) against the definition, value by value; got"""
+    q = bnd.held_in(s.torch, kind, q)
+    scale = s.hd ** -0.5 if scale is None else scale
+    got, row = s.attend(entries, q, kind, scale, n_sel), 0
+    got, blocks = got if n_sel else (got, None)
+    for slot, pos0, rows in entries:
+        for pos in range(pos0, pos0 + rows):
+            seen = None
+            if n_sel:
+                assert np.array_equal(blocks[row], orc.selected(s.k[slot], q[row], pos, n_sel)), (slot, pos)
+                seen = bnd.seen_of(blocks[row], pos)
+            want, tol = bnd.attention(q[row], s.k[slot, :pos + 1], s.v[slot, :pos + 1], scale, kind, prompt, seen)
+            far = bnd.far(got[row], want, tol)
+            assert far <= 1, (slot, pos, far)
+            row += 1
+    return got
 
 
 def test_near_constant_groups(cuda):
@@ -30,4 +51,38 @@ def test_near_constant_groups(cuda):
     s.write([(0, 0, x.shape[0])], x, x[::-1])
     gk, gv = s.read([(0, 0, x.shape[0])])
     assert np.array_equal(gk, s.k[0]) and np.array_equal(gv, s.v[0])
+    s.close()
+
+
+def test_f32_rows_over_wide_values(cuda):
+    """value groups up to f16's limits (m + 15 d up to 16 x 65504) among ordinary ones, at positions that rows see and at
+    positions of the same record that they do not"""
+    rng = np.random.default_rng(32)
+    s = Session(cuda, 1, 4, 2, 128, 300)
+    k, v = _rows(rng, 300, 2, 128)
+    v[70, 0, 5], v[70, 1, 40], v[200, 0, 64:96] = 2e5, -6e4, np.linspace(65504, 65504 * 16, 32)
+    v[130, 1, 96:] = np.linspace(-65504, 65504 * 14, 32)
+    s.write([(0, 0, 300)], k, v)
+    assert np.isfinite(s.v).all() and s.v.max() > 1e6
+    q = rng.normal(size=(8, 4, 128)).astype(np.float32)
+    for entries in ([(0, 69, 1), (0, 70, 1), (0, 71, 1), (0, 128, 2), (0, 199, 2), (0, 299, 1)], [(0, 64, 8)], [(0, 196, 8)]):
+        n = sum(e[2] for e in entries)
+        _check(s, entries, q[:n], "f32")
+        _check(s, entries, q[:n], "f32", n_sel=2)
+    got = s.s.decode(0, 0, 299, q[0], k[299], v[299], 0.1)
+    want, tol = bnd.attention(q[0], s.k[0], s.v[0], 0.1, "f32")
+    assert bnd.far(got, want, tol) <= 1
+    s.s.check()
+    s.close()
+
+
+def test_f32_rows_over_small_values(cuda):
+    """values of every size down to f16's smallest scales: what the minimum's two parts drop is relative to them"""
+    rng = np.random.default_rng(33)
+    s = Session(cuda, 1, 2, 2, 128, 500)
+    for size in (1e-2, 1e-4, 3e-6):
+        k, v = _rows(rng, 500, 2, 128)
+        v[:, :, 32:] *= size
+        s.write([(0, 0, 500)], k, v)
+        _check(s, [(0, 499, 1), (0, 33, 1)], rng.normal(size=(2, 2, 128)), "f32")
     s.close()

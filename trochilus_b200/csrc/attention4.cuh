@@ -874,14 +874,16 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 // rows 0 .. NG - 1 of A are the groups' minima, row NG ones
                 m[k] = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VM + (8 * t + 4 * k + cc) * (NG * 4) + n * 4)
                               : n == NG ? 0x3c003c00u : 0u;
-                // m + 8 d, and (rows n + 8) what its rounding drops; a NaN belongs to every row where all see the position
+                // (m + 8 d) / 16, which f16 holds for every m and d, and (rows n + 8) what 16 times its rounding drops: no
+                // smaller than f16's smallest numbers, of which m and 8 d are multiples; a NaN belongs to every row where
+                // all see the position
                 if constexpr (MID != 0) {
                     const uint32_t x = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VD + (8 * t + 4 * k + cc) * (NG * 4) + n * 4) : 0u;
                     const float2 md = trx_a4_float2(m[k]), dd = trx_a4_float2(MASK ? trx_a4_finite(x) : x);
                     const float y = __fmaf_rn(dd.x, (float)MID, md.x), z = __fmaf_rn(dd.y, (float)MID, md.y);
-                    m[k] = trx_a4_half2(y, z);
+                    m[k] = trx_a4_half2(y * 0.0625f, z * 0.0625f);
                     const float2 r = trx_a4_float2(m[k]);
-                    ml[k] = trx_a4_half2(y - r.x, z - r.y);
+                    ml[k] = trx_a4_half2(__fmaf_rn(r.x, -16.0f, y), __fmaf_rn(r.y, -16.0f, z));
                 }
 #pragma unroll
                 for (int r = 0; r < NT; r++) {
@@ -938,10 +940,11 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
             for (int i = 0; i < 2; i++) { // query row 2 cc + i
                 const int row = 8 * r + 2 * cc + i;
                 if (n == 0) refs[row] = ref[r][i];
-                if (n == NG) sums[row] = accm[r][i];
+                const float own = MID ? __fmaf_rn(accm[r][i], 16.0f, accm[r][2 + i]) : accm[r][i]; // a group's minima, or ones
+                if (n == NG) sums[row] = own;
 #pragma unroll
                 for (int g = 0; g < NG; g++) { // dims 32 g + 4 n + 0..3
-                    const float m = __shfl_sync(0xffffffffu, MID ? accm[r][i] + accm[r][2 + i] : accm[r][i], 4 * g + cc);
+                    const float m = __shfl_sync(0xffffffffu, own, 4 * g + cc);
                     const float e = EXACT ? 1.0f : 16777216.0f, f = EXACT ? 1.0f : 1048576.0f; // 2^24, 2^20
                     *reinterpret_cast<float4 *>(o + row * HD + 32 * g + 4 * n) =
                         make_float4(__fmaf_rn(acc[g][0][r][i], e, m), __fmaf_rn(acc[g][0][r][2 + i], f, m),
