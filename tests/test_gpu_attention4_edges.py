@@ -29,6 +29,12 @@ def _check(s, entries, q, kind, scale=None, n_sel=None, prompt=False):
     return got
 
 
+def _prompt(s, rows, kind, entries=2):
+    """entries of `rows` rows from position 0 on, enough for the prompt kernel"""
+    assert kind != "f32" and bnd.takes_prompt_kernel(s.torch, entries, rows, s.heads, s.kv)
+    return [(i, 0, rows) for i in range(entries)]
+
+
 def test_near_constant_groups(cuda):
     """groups whose values differ by less than their minimum's last place: scales among f16's smallest numbers, rounded by
     up to a third, so that quotients pass 15"""
@@ -85,4 +91,24 @@ def test_f32_rows_over_small_values(cuda):
         v[:, :, 32:] *= size
         s.write([(0, 0, 500)], k, v)
         _check(s, [(0, 499, 1), (0, 33, 1)], rng.normal(size=(2, 2, 128)), "f32")
+    s.close()
+
+
+@pytest.mark.parametrize("kind", ("bf16", "f16"))
+def test_prompt_rows_that_are_not_finite(cuda, kind):
+    """a query row with a NaN or an infinity among a prompt's is NaN in its head, and in no other row or head"""
+    rng = np.random.default_rng(34)
+    s = Session(cuda, 2, 32, 4, 128, 260)
+    s.write([(0, 0, 260), (1, 0, 260)], *_rows(rng, 520, 4, 128), kind)
+    q = rng.normal(size=(520, 32, 128)).astype(np.float32)
+    entries = _prompt(s, 260, kind)
+    clean = s.attend(entries, q, kind)
+    bad = ((0, 3, 5), (17, 0, 0), (100, 31, 127), (259, 9, 64), (260, 8, 1), (400, 16, 33))
+    for i, (r, h, x) in enumerate(bad):
+        q[r, h, x] = (np.nan, np.inf, -np.inf)[i % 3]
+    got = s.attend(entries, q, kind)
+    for r, h, _ in bad:
+        assert np.isnan(got[r, h]).all(), (r, h)
+        got[r, h] = clean[r, h]
+    assert np.array_equal(got, clean)
     s.close()

@@ -242,7 +242,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
             // ---- softmax
             const int n = n_tiles[t_mine];
             const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + 128 * t_mine, to = ts + 256;
-            const float c = fminf(c0 * __int_as_float((ek + 127) << 23), 3.0e38f);
+            const float f = c0 * __int_as_float((ek + 127) << 23), c = f > 3.0e38f ? 3.0e38f : f; // (a NaN stays)
             float top = -1.0e30f, ref = -1.0e30f;
             trx_f2 sum = 0;
             const int low = __reduce_min_sync(0xffffffffu, lim);
