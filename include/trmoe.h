@@ -363,7 +363,8 @@ TRMOE_API int tr_gpu_attn4_read_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu
  * or drafted tokens. q and out [n_tok][n_head * head_dim]. Scores and sums are in 32 bits, and so is the rest for f32
  * rows (two 16-bit parts of each factor); for 16-bit rows a probability is rounded to f16 (2^-12 relative), and in calls
  * of many rows the keys and values are. A NaN or an infinity among the positions that a row sees makes that head's
- * output, or its group of 32 values, NaN; among others it does not matter. */
+ * output, or its group of 32 values, NaN; among others it does not matter. One in a head's q makes that head's output
+ * NaN, one as scale every output. */
 TRMOE_API int tr_gpu_attn4_attend_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type,
                                       const void *q, int64_t q_stride, float scale, void *out, int64_t out_stride,
                                       void *stream);

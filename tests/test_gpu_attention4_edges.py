@@ -5,7 +5,7 @@ import pytest
 
 from tests import attn4_bounds as bnd
 from tests import attn4_oracle as orc
-from tests.test_gpu_attention4 import Session, _rows
+from tests.test_gpu_attention4 import KINDS, Session, _rows
 
 pytestmark = pytest.mark.gpu
 
@@ -111,4 +111,22 @@ def test_prompt_rows_that_are_not_finite(cuda, kind):
         assert np.isnan(got[r, h]).all(), (r, h)
         got[r, h] = clean[r, h]
     assert np.array_equal(got, clean)
+    s.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_scales_that_are_not_finite(cuda, kind):
+    """a NaN or an infinity as scale gives NaN, whichever kernel a call takes"""
+    rng = np.random.default_rng(35)
+    s = Session(cuda, 2, 32, 4, 128, 260)
+    s.write([(0, 0, 260), (1, 0, 260)], *_rows(rng, 520, 4, 128), kind)
+    q = rng.normal(size=(520, 32, 128)).astype(np.float32)
+    for scale in (np.nan, np.inf, -np.inf):
+        assert np.isnan(s.attend([(0, 259, 1), (1, 0, 1)], q[:2], kind, scale)).all()
+        out, blocks = s.attend([(0, 259, 1), (1, 0, 1)], q[:2], kind, scale, n_sel=2)
+        assert np.isnan(out).all() and np.array_equal(blocks, s.attend([(0, 259, 1), (1, 0, 1)], q[:2], kind, 1.0, n_sel=2)[1])
+        if kind != "f32":
+            assert np.isnan(s.attend(_prompt(s, 260, kind), q, kind, scale)).all()
+    if kind == "f32":
+        assert np.isnan(s.s.decode(0, 0, 259, q[0], s.k[0, 259], s.v[0, 259], np.nan)).all()
     s.close()

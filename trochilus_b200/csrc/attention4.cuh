@@ -678,7 +678,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
             // (2^24: the codes are subnormals; capped, so that a score of 0 stays 0)
             float factor = fminf(fabsf(scale) * 1.44269504088896341f *
                                      __int_as_float((min(ex, 113) + (EXACT ? -10 : 14) + 127) << 23), 3.0e38f);
-            if (bad) factor = __int_as_float(0x7fffffff);
+            if (bad || !(fabsf(scale) <= 3.402823466e38f)) factor = __int_as_float(0x7fffffff);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 c[t][i] = __shfl_sync(0xffffffffu, factor, 4 * (2 * cc + i));
