@@ -130,3 +130,18 @@ def test_scales_that_are_not_finite(cuda, kind):
     if kind == "f32":
         assert np.isnan(s.s.decode(0, 0, 259, q[0], s.k[0, 259], s.v[0, 259], np.nan)).all()
     s.close()
+
+
+@pytest.mark.parametrize("kind", ("f32", "bf16"))
+def test_queries_near_the_largest_number(cuda, kind):
+    """queries of 2^112 to 2^127 whose scale brings the scores back"""
+    rng = np.random.default_rng(36)
+    s = Session(cuda, 2, 32, 4, 128, 260)
+    s.write([(0, 0, 260), (1, 0, 260)], *_rows(rng, 520, 4, 128), kind)
+    q = rng.normal(size=(520, 32, 128)).astype(np.float32)
+    for size in (112, 114, 120, 124):
+        _check(s, [(0, 259, 1), (1, 100, 1)], np.ldexp(q[:2], size), kind, 0.1 * 2.0 ** -size)
+    if kind != "f32":
+        _prompt(s, 260, kind)
+        _check(s, [(0, 0, 260), (1, 0, 260)], np.ldexp(q, 122), kind, 0.1 * 2.0 ** -122, prompt=True)
+    s.close()

@@ -675,9 +675,10 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
             int ex = 0;
             if (!bad && most > 0.0f) ex = max((int)((__float_as_uint(most) >> 23) & 255) - 126, -100);
             const float f = __int_as_float((10 - ex + 127) << 23) * (scale < 0.0f ? -1.0f : 1.0f);
-            // (2^24: the codes are subnormals; capped, so that a score of 0 stays 0)
-            float factor = fminf(fabsf(scale) * 1.44269504088896341f *
-                                     __int_as_float((min(ex, 113) + (EXACT ? -10 : 14) + 127) << 23), 3.0e38f);
+            // (in two steps, as 2^(ex + 14) may pass 32 bits: 2^24, where the codes are subnormals; capped, so that a score
+            // of 0 stays 0)
+            float factor = fminf(fabsf(scale) * (1.44269504088896341f * __int_as_float((ex - 10 + 127) << 23)) *
+                                     (EXACT ? 1.0f : 16777216.0f), 3.0e38f);
             if (bad || !(fabsf(scale) <= 3.402823466e38f)) factor = __int_as_float(0x7fffffff);
 #pragma unroll
             for (int i = 0; i < 2; i++) {

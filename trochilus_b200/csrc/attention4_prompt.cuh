@@ -188,7 +188,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
         // (kept above 0 and in range: a masked score, -inf, stays one and a score of 0 stays 0)
         c0 = bad || !(fabsf(scale) <= 3.402823466e38f)
                  ? __int_as_float(0x7fffffff)
-                 : fminf(1.0e-30f + fabsf(scale) * 1.44269504088896341f * __int_as_float((min(ex, 120) - 10 + 127) << 23), 3.0e36f);
+                 : fminf(1.0e-30f + fabsf(scale) * (1.44269504088896341f * __int_as_float((ex - 10 + 127) << 23)), 3.0e36f);
 #pragma unroll
         for (int i = 0; i < HD / 8; i++) { // (dims 32 g + 8 c ..: chunk 4 g + c)
             const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
