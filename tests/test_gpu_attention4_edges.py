@@ -35,6 +35,20 @@ def _prompt(s, rows, kind, entries=2):
     return [(i, 0, rows) for i in range(entries)]
 
 
+def _single(s, entries, q, kind, scale, n_sel=None):
+    """rows of which one position has all the weight: its value, to the output's rounding (prompts': and f16's)"""
+    got, row = s.attend(entries, q, kind, scale, n_sel), 0
+    got = got[0] if n_sel else got
+    for slot, pos0, rows in entries:
+        for pos in range(pos0, pos0 + rows):
+            want = np.repeat(s.v[slot, pos], s.heads // s.kv, 0)
+            size = np.repeat(abs(want).reshape(s.heads, -1, 32).max(-1), 32, -1).reshape(want.shape)
+            tol = size * ((2.0 ** -17 if kind == "f32" else 5 * 2.0 ** -11) + bnd.HALF_STEP[kind])
+            far = bnd.far(got[row], want, tol)
+            assert far <= 1, (slot, pos, scale, far)
+            row += 1
+
+
 def test_near_constant_groups(cuda):
     """groups whose values differ by less than their minimum's last place: scales among f16's smallest numbers, rounded by
     up to a third, so that quotients pass 15"""
@@ -144,4 +158,28 @@ def test_queries_near_the_largest_number(cuda, kind):
     if kind != "f32":
         _prompt(s, 260, kind)
         _check(s, [(0, 0, 260), (1, 0, 260)], np.ldexp(q, 122), kind, 0.1 * 2.0 ** -122, prompt=True)
+    s.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_scores_past_a_million(cuda, kind):
+    """scores whose neighbours in 32 bits lie further apart than a softmax can tell: the best position has all the weight"""
+    rng = np.random.default_rng(37)
+    s = Session(cuda, 2, 32, 4, 128, 260)
+    k, v = _rows(rng, 520, 4, 128)
+    k[:] = np.sign(rng.normal(size=k.shape)) * (1 + np.arange(520) % 260)[:, None, None] / 260  # the later, the larger
+    s.write([(0, 0, 260), (1, 0, 260)], k, v, kind)
+    q = np.sign(rng.normal(size=(520, 32, 128))).astype(np.float32)
+    for i in range(2):
+        for r in range(260):
+            q[260 * i + r] = np.repeat(np.sign(s.k[i, r]), 8, 0) + 0.0  # (its own key: no other is as large)
+    for size in (1e5, 1e6, 3e6, 1e7, 3e7, 1e8, 1e9):
+        scale = size / 128
+        _single(s, [(0, 259, 1), (1, 0, 1), (1, 33, 1), (0, 100, 3)], q[[259, 260, 293, 100, 101, 102]], kind, scale)
+        _single(s, [(0, 259, 1), (1, 200, 1)], q[[259, 460]], kind, scale, n_sel=2)
+        if kind != "f32" and size <= 1e8:
+            _single(s, _prompt(s, 260, kind), q, kind, scale)
+    # scores that are all far below zero: the least far has the weight, and a row's first position sees itself alone
+    for size in (1e8, 1e34, 1e36) if kind != "f16" else (1e8,):
+        _single(s, [(0, 0, 1), (1, 0, 1)], -q[[0, 260]], kind, size / 128)
     s.close()

@@ -637,6 +637,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
     static_assert(R == 8 || (R == 16 && !F32), "8 rows, or 16 of a 16-bit type");
     // scores of 16-bit types may pass the reference by 2^LAZY before the sums are rescaled
     static constexpr float LAZY = F32 ? 0.0f : 8.0f, TOP = F32 ? 14.0f : 7.0f;
+    static constexpr float NONE = -3.0e38f; // the maximum of a row that has seen no position
     uint32_t qb[NB][2 * NG][2]; // the query fragments: lane (n = lane / 4, c = lane % 4) has row n (+ 8)
     uint32_t qs[NT];            // their groups' sums
     int lim[NT];                // the last position row n (+ 8) sees; -1: no row
@@ -683,7 +684,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 c[t][i] = __shfl_sync(0xffffffffu, factor, 4 * (2 * cc + i));
-                top[t][i] = ref[t][i] = -1.0e30f;
+                top[t][i] = ref[t][i] = NONE;
             }
 #pragma unroll
             for (int g = 0; g < NG; g++) {
@@ -818,7 +819,8 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                         if (MASK && pos0 + 16 * t + 8 * k + n > last) x = -INFINITY;
                         best = fmaxf(best, x);
                     }
-                grow |= best > top[r][i] + LAZY;
+                // (rounded down, as the reference is rounded up: p must not pass f16 where scores of 2^25 and more lie apart)
+                grow |= best > __fadd_rd(top[r][i], LAZY);
                 f[r][i] = best;
             }
         }
@@ -836,7 +838,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
                     for (int x = 4; x <= 16; x <<= 1) f[r][i] = fmaxf(f[r][i], __shfl_xor_sync(0xffffffffu, f[r][i], x));
                     top[r][i] = fmaxf(top[r][i], f[r][i]);
-                    const float to = top[r][i] == -1.0e30f ? -1.0e30f : top[r][i] + ed - TOP;
+                    const float to = top[r][i] == NONE ? NONE : __fadd_ru(top[r][i], ed - TOP);
                     f[r][i] = ref[r][i] == to ? 1.0f : trx_a4_exp2(ref[r][i] - to);
                     ref[r][i] = to;
                 }

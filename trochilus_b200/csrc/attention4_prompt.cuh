@@ -24,6 +24,9 @@
 // The keys' and values' rounding to f16 (2^-12 relative) is the choice that the 16-bit rows allow: half a step of f16
 // rows, a sixteenth of bf16's. Values past f16 (|m| + 15 d > 60000, which a cache of bf16 or f32 rows may hold) make the
 // CTA start again with all keys and all values multiplied by a power of two that fits the largest of its context.
+// Scores of 2^22 and more (log2) make it start again too, with each product of a score and its factor rounded as the
+// maximum's is: what a fused one keeps beside the reference would let p pass f16 from 2^24 on. (Rounding them always: 309 us
+// for 296.)
 // A NaN among the values must not reach the rows that do not see its position, though their p is 0: it is written as 0,
 // and the first position of such a group is kept; rows that see it get NaN at the end.
 #pragma once
@@ -135,7 +138,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
     extern __shared__ __align__(128) uint8_t smem_raw[];
     __shared__ __align__(8) TrxA4PBars bar;
     __shared__ uint32_t s_tmem;
-    __shared__ int s_fail, s_wide, s_nan[NG], s_most[2];
+    __shared__ int s_fail, s_again, s_nan[NG], s_most[2];
     int slot, row0, rows, pos0;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kv = blockIdx.x % a.n_kv, G = a.n_head / a.n_kv;
     if (!trx_a4_entry(a, b, blockIdx.z, slot, row0, rows, pos0)) return;
@@ -208,7 +211,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
         trx_tmem_alloc(&s_tmem, 512);
         trx_tmem_relinquish();
     }
-    if (tid == 0) s_fail = 0, s_wide = 0, s_most[0] = s_most[1] = 0;
+    if (tid == 0) s_fail = 0, s_again = 0, s_most[0] = s_most[1] = 0;
     if (tid < NG) s_nan[tid] = INT_MAX;
 
     float l = 0.0f;
@@ -244,67 +247,78 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
             const int n = n_tiles[t_mine];
             const uint32_t ts = tmem + ((uint32_t)(warp & 3) << 21) + 128 * t_mine, to = ts + 256;
             const float f = c0 * __int_as_float((ek + 127) << 23), c = f > 3.0e38f ? 3.0e38f : f; // (a NaN stays)
-            float top = -1.0e30f, ref = -1.0e30f;
+            constexpr float NONE = -3.0e38f; // no position seen
+            float top = NONE, ref = NONE;
             trx_f2 sum = 0;
             const int low = __reduce_min_sync(0xffffffffu, lim);
-            for (int j = 0; j < n; j++) {
-                if (!__all_sync(0xffffffffu, wait(&bar.s_full[t_mine], j))) break;
-                trx_tc_fence_after();
-                const bool mask = j * KT + KT - 1 > low;
-                const int see = lim - j * KT; // the tile's last column that the row sees
-                // 32 columns from `at`: their maximum, and p
-                auto look = [&](uint32_t(&r)[32], int at) {
-                    if (mask) {
+            // FAR: the products s c are rounded, as the maximum's is, before the reference is subtracted
+            auto tiles = [&](auto far) {
+                constexpr bool FAR = decltype(far)::value;
+                for (int j = 0; j < n; j++) {
+                    if (!__all_sync(0xffffffffu, wait(&bar.s_full[t_mine], j))) break;
+                    trx_tc_fence_after();
+                    const bool mask = j * KT + KT - 1 > low;
+                    const int see = lim - j * KT; // the tile's last column that the row sees
+                    // 32 columns from `at`: their maximum, and p
+                    auto look = [&](uint32_t(&r)[32], int at) {
+                        if (mask) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) // (volatile: a branch, not 32 selections for every tile)
-                            asm volatile("{\n .reg .pred q;\n setp.gt.s32 q, %1, %2;\n @q mov.b32 %0, 0xff800000;\n}"
-                                         : "+r"(r[i])
-                                         : "r"(at + i), "r"(see));
-                    }
-                    float best[4];
+                            for (int i = 0; i < 32; i++) // (volatile: a branch, not 32 selections for every tile)
+                                asm volatile("{\n .reg .pred q;\n setp.gt.s32 q, %1, %2;\n @q mov.b32 %0, 0xff800000;\n}"
+                                             : "+r"(r[i])
+                                             : "r"(at + i), "r"(see));
+                        }
+                        float best[4];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        best[k] = fmaxf(__uint_as_float(r[8 * k]), __uint_as_float(r[8 * k + 1]));
+                        for (int k = 0; k < 4; k++) {
+                            best[k] = fmaxf(__uint_as_float(r[8 * k]), __uint_as_float(r[8 * k + 1]));
 #pragma unroll
-                        for (int i = 2; i < 8; i += 2)
-                            best[k] = trx_a4_max3(best[k], __uint_as_float(r[8 * k + i]), __uint_as_float(r[8 * k + i + 1]));
-                    }
-                    return trx_a4_max3(fmaxf(best[0], best[1]), best[2], best[3]) * c;
-                };
-                auto take = [&](uint32_t(&r)[32], int at) {
-                    uint32_t p[16];
+                            for (int i = 2; i < 8; i += 2)
+                                best[k] = trx_a4_max3(best[k], __uint_as_float(r[8 * k + i]), __uint_as_float(r[8 * k + i + 1]));
+                        }
+                        return trx_a4_max3(fmaxf(best[0], best[1]), best[2], best[3]) * c;
+                    };
+                    auto take = [&](uint32_t(&r)[32], int at) {
+                        uint32_t p[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const trx_f2 e = trx_fma2((trx_f2)r[i] | (trx_f2)r[i + 1] << 32, trx_pack2(c, c), trx_pack2(-ref, -ref));
-                        const float x = trx_a4_exp2(trx_lo(e)), y = trx_a4_exp2(trx_hi(e));
-                        p[i / 2] = trx_a4_half2(x, y);
-                        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(trx_pack2(x, y)));
-                    }
-                    trx_a4p_st16(ts + at / 2, p);
-                };
+                        for (int i = 0; i < 32; i += 2) {
+                            trx_f2 e = (trx_f2)r[i] | (trx_f2)r[i + 1] << 32;
+                            if constexpr (FAR) e = trx_sub2(trx_mul2(e, trx_pack2(c, c)), trx_pack2(ref, ref));
+                            else e = trx_fma2(e, trx_pack2(c, c), trx_pack2(-ref, -ref));
+                            const float x = trx_a4_exp2(trx_lo(e)), y = trx_a4_exp2(trx_hi(e));
+                            p[i / 2] = trx_a4_half2(x, y);
+                            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum) : "l"(trx_pack2(x, y)));
+                        }
+                        trx_a4p_st16(ts + at / 2, p);
+                    };
 #pragma unroll 1
-                for (int h = 0; h < 128; h += 64) {
-                    uint32_t r0[32], r1[32];
-                    trx_tmem_ld32_nw(ts + h, r0);
-                    trx_tmem_ld32_nw(ts + h + 32, r1);
-                    trx_a4p_landed(r0);
-                    trx_a4p_landed(r1);
-                    const float best = fmaxf(look(r0, h), look(r1, h + 32));
-                    if (__any_sync(0xffffffffu, best > top + 8.0f)) { // (S j is complete: so are O's products before it)
-                        top = fmaxf(top, best);
-                        const float next = top == -1.0e30f ? -1.0e30f : top - 7.0f, f = ref == next ? 1.0f : trx_a4_exp2(ref - next);
-                        ref = next;
-                        sum = trx_mul2(sum, trx_pack2(f, f));
-                        trx_a4p_rescale(to, j > 0 ? HD : 0, ts, h / 2, f);
+                    for (int h = 0; h < 128; h += 64) {
+                        uint32_t r0[32], r1[32];
+                        trx_tmem_ld32_nw(ts + h, r0);
+                        trx_tmem_ld32_nw(ts + h + 32, r1);
+                        trx_a4p_landed(r0);
+                        trx_a4p_landed(r1);
+                        const float best = fmaxf(look(r0, h), look(r1, h + 32));
+                        if (__any_sync(0xffffffffu, best > __fadd_rd(top, 8.0f))) { // (S j is complete: so are O's products before it)
+                            top = fmaxf(top, best);
+                            // (rounded up, and 8 more rounded down: p must not pass f16 where scores are large)
+                            const float next = top == NONE ? NONE : __fadd_ru(top, -7.0f), f = ref == next ? 1.0f : trx_a4_exp2(ref - next);
+                            if (!FAR && fabsf(top) >= 4194304.0f && top != NONE) *(volatile int *)&s_again = 1;
+                            ref = next;
+                            sum = trx_mul2(sum, trx_pack2(f, f));
+                            trx_a4p_rescale(to, j > 0 ? HD : 0, ts, h / 2, f);
+                        }
+                        take(r0, h);
+                        take(r1, h + 32); // (S's columns h / 2 .. h / 2 + 31 have been read)
                     }
-                    take(r0, h);
-                    take(r1, h + 32); // (S's columns h / 2 .. h / 2 + 31 have been read)
+                    trx_tmem_wait_st();
+                    trx_tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) trx_a4p_arrive(&bar.p_ready[t_mine]);
                 }
-                trx_tmem_wait_st();
-                trx_tc_fence_before();
-                __syncwarp();
-                if (lane == 0) trx_a4p_arrive(&bar.p_ready[t_mine]);
-            }
+            };
+            if (attempt == 0) tiles(std::false_type{});
+            else tiles(std::true_type{});
             l = trx_lo(sum) + trx_hi(sum);
             if (n > 0) __all_sync(0xffffffffu, wait(&bar.o_full[t_mine], 0));
             trx_tc_fence_after();
@@ -352,7 +366,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                         trx_a4p_ends(x.d[g], x.m[g], hi, lo);
                     }
                 }
-                if (trx_a4p_wide(hi, lo)) *(volatile int *)&s_wide = 1;
+                if (trx_a4p_wide(hi, lo)) *(volatile int *)&s_again = 1;
                 const uint32_t to = rows + st * S::K + (t8 >> 3) * (HD * 128) + (((t8 & 7) ^ (lane & 7)) << 4);
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
@@ -405,7 +419,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
                     trx_a4p_ends(x.d[i], x.m[i], hi, lo); // (beside a NaN: its scores are NaN)
                     if (ek) x.d[i] = trx_a4_hmul2(x.d[i], hk), x.m[i] = trx_a4_hmul2(x.m[i], hk);
                 }
-                if (trx_a4p_wide(hi, lo)) *(volatile int *)&s_wide = 1;
+                if (trx_a4p_wide(hi, lo)) *(volatile int *)&s_again = 1;
                 uint8_t *to = sk + st * S::K;
 #pragma unroll
                 for (int g = 0; g < NG; g++) {
@@ -483,7 +497,7 @@ template <int HD> __global__ void __launch_bounds__(TRX_A4P_THREADS, 1)
         trx_tc_fence_before();
         __syncthreads();
         trx_tc_fence_after();
-        if (attempt > 0 || *(volatile int *)&s_wide == 0 || *(volatile int *)&s_fail != 0) break;
+        if (attempt > 0 || *(volatile int *)&s_again == 0 || *(volatile int *)&s_fail != 0) break;
         // the largest |m| + 15 d of the keys and of the values
         float most[2] = {0.0f, 0.0f};
         const int words = 16 * NG; // of a plane
