@@ -27,9 +27,10 @@ def attention(q, k, v, scale, kind, prompt=False, seen=None):
       the tensor core's sums of subnormal codes drop at most 2^-13 of 15 d; prompts round the values instead (2^-11 M_t
       and 2^-25). Together 5 x 2^-11 sum p_t M_t.
     - f32 rows: p and p d in two parts each 2^-21, the minimum's term 2^-21, additions: 2^-17 sum p_t M_t holds them.
-    - what f16 drops below its smallest number: 2^-25 of p, whose largest is at least 2^7 (f32 rows 2^14) over the largest
-      value scale above 1: 2^(ed - 32) x 3 M_t a position (f32: 2^(ed - 39)); and of p d, where a group's scales below
-      2^-8 are multiplied up to 1: 15 x 2^-32 x min(1, 2^8 x the group's largest d <= 2 M / 15) a position.
+    - what f16 drops below its smallest number: 2^-25 of p, whose largest is at least 2^7 (f32 rows 2^14) over 2^ed, ed the
+      binary logarithm of the KV head's largest value scale where that is above 1: 2^(ed - 32) x 3 M_t a position (f32: 2^(ed -
+      39)); and as much of each code's share 15 p d, where scales below 2^-8 are multiplied up to 1: 15 x 2^(ed - 32) x min(1,
+      2^8 x the KV head's largest d) a position (d <= 2 M / 15).
     - the output's rounding: half a step, or 2^-25 below f16's normal numbers."""
     kv = k.shape[1]
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
@@ -48,11 +49,13 @@ def attention(q, k, v, scale, kind, prompt=False, seen=None):
     m = abs(v).reshape(n, kv, -1, 32).max(-1)
     weight = p * (2 * np.where(p > 0, off, 0) + (2.0 ** -17 if kind == "f32" else 5 * 2.0 ** -11))
     tol = np.einsum("hgt,thx->hgx", weight, m)
-    span = np.maximum(v.reshape(n, kv, -1, 32).max(-1) - v.reshape(n, kv, -1, 32).min(-1), 0).max() / 15
-    ed = 0 if prompt else max(0, int(np.frexp(span)[1]))
-    tol += 2.0 ** (ed - (39 if kind == "f32" else 32)) * 3 * m.sum(0)[:, None]
     if not prompt:
-        tol += n * 15 * 2.0 ** -32 * np.minimum(1, 256 * 2 * m.max(0) / 15)[:, None]
+        x = v.reshape(n, kv, -1, 32)
+        d = (x.max(-1) - x.min(-1)).max((0, 2)) / 15  # (KV heads)
+        low = 2.0 ** (np.maximum(0, np.frexp(d)[1]) - (39.0 if kind == "f32" else 32.0))
+        tol += low[:, None, None] * (3 * m.sum(0) + n * 15 * np.minimum(1, 256 * d)[:, None])[:, None]
+    else:
+        tol += 2.0 ** -32 * 3 * m.sum(0)[:, None]
     tol = np.repeat(tol, 32, -1) + abs(out) * HALF_STEP[kind] + (2.0 ** -25 if kind == "f16" else 0) + 1e-37
     return out.reshape(q.shape), tol.reshape(q.shape)
 

@@ -183,3 +183,40 @@ def test_scores_past_a_million(cuda, kind):
     for size in (1e8, 1e34, 1e36) if kind != "f16" else (1e8,):
         _single(s, [(0, 0, 1), (1, 0, 1)], -q[[0, 260]], kind, size / 128)
     s.close()
+
+
+@pytest.mark.parametrize("size,sink,kind", [(1e-5, 20, "f32"), *[(size, 16, kind) for size in (1e-3, 1e-4, 3e-5) for kind in KINDS]])
+def test_small_values_behind_a_sink(cuda, size, sink, kind):
+    """values whose scales are f16's smallest, and one position whose weight is 2^sink times the others': what the others
+    add is not lost"""
+    rng = np.random.default_rng(38)
+    n = 8192
+    s = Session(cuda, 1, 2, 2, 128, n)
+    k = (0.05 * rng.normal(size=(n, 2, 128))).astype(np.float32)
+    v = (size * (1 + rng.normal(size=(n, 2, 128)))).astype(np.float32)
+    q = np.sign(rng.normal(size=(1, 2, 128))).astype(np.float32)
+    k[5] = q[0] * (sink * np.log(2) * 128 ** -0.5)
+    v[5] *= 0.01
+    s.write([(0, 0, n)], k, v, kind)
+    got = _check(s, [(0, n - 1, 1)], q, kind)[0]
+    want, _ = bnd.attention(bnd.held_in(cuda, kind, q)[0], s.k[0], s.v[0], 128 ** -0.5, kind)
+    # f16 outputs of this size lie 2^-24 apart
+    tol = np.linalg.norm(want) * {"f32": 2.0 ** -14, "bf16": 2.0 ** -8, "f16": 2.0 ** -10}[kind]
+    assert np.linalg.norm(got - want) <= tol + (2.0 ** -25 * 16 if kind == "f16" else 0)
+    s.close()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_values_that_grow(cuda, kind):
+    """value scales that grow through 2^-24 .. 2^4 along a sequence, whose sums change their units on the way"""
+    rng = np.random.default_rng(39)
+    n = 4096
+    s = Session(cuda, 1, 16, 2, 64, n)
+    k, v = _rows(rng, n, 2, 64)
+    v *= np.ldexp(1.0, -22 + np.arange(n) // 150)[:, None, None].astype(np.float32)
+    s.write([(0, 0, n)], k, v, kind)
+    q = 0.5 * rng.normal(size=(3, 16, 64))
+    for at in (100, 700, 1700, 2400, 3300, n - 3):
+        _check(s, [(0, at, 1), (0, at, 2)], q, kind)
+        _check(s, [(0, at, 1), (0, at, 2)], q, kind, n_sel=5)
+    s.close()

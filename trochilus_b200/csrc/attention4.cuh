@@ -465,7 +465,9 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 //            ones, which sum p) as A.
 // 16 query rows of f16 or bf16 type, or 8 (R), share the codes' unpacking; scores, sums and outputs are f32.
 // p stays below 2^15 / max(1, d): the reference that is subtracted in the exponent is the row's maximum so far, plus
-// the binary logarithm of the largest value scale so far where it is above 1, less a constant.
+// the binary logarithm of the largest value scale so far where it is above 1, less a constant. Where all scales so far are
+// below 2^-8 they are multiplied up to 1: without it, values of 3e-5 behind a position of 2^16 times their weight came out
+// 3e-2 off.
 //
 // A cluster of CTAs shares one tile of query rows: its warps take records in turn, their results are joined in each
 // CTA through shared memory, and the CTAs' through distributed shared memory, so that no workspace or second launch is
@@ -643,7 +645,10 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
     int lim[NT];                // the last position row n (+ 8) sees; -1: no row
     float c[NT][2];             // rows 2 c, 2 c + 1 (+ 8): the scores' factor, with log2(e),
     float top[NT][2], ref[NT][2]; // the running maximum, and what the exponent subtracts
-    float ed, edlim;            // binary logarithm of the largest value scale so far, at least 0, and its power
+    // 2^ed = edlim is above the largest value scale so far: from 2^-8 on at least 1, and the references take it up; below,
+    // scales are multiplied by 2^-ed (small values' products with p would be among f16's smallest numbers, or 0)
+    int ed;
+    float edlim;
     float acc[NG][2][NT][4], accm[NT][4];
 
     // the query rows of the tile: row r of it is at off(r); rows past n_rows are zero
@@ -729,11 +734,11 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
                     for (int i = 0; i < 4; i++) acc[g][h][t][i] = 0.0f;
         }
-        ed = 0.0f, edlim = 1.0f;
+        ed = -15, edlim = 3.0517578125e-5f;
     }
 
     // one record (32 positions from pos0); MASK: some row does not see all of them
-    template <bool MASK> __device__ __forceinline__ void record(const uint8_t *rec, int lane, int pos0) {
+    template <bool MASK> __device__ __forceinline__ void record(uint8_t *rec, int lane, int pos0) {
         using L = TrxA4L<HD>;
         const int n = lane >> 2, cc = lane & 3;
         float s[2][NT][4]; // 16 positions each: n (0, 1) and n + 8 (2, 3) x rows 2 cc, 2 cc + 1
@@ -827,9 +832,12 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
             for (int x = 1; x <= 16; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+            float units = 1.0f; // the outputs' by the scales' multiplier
             if (big > edlim) {
-                const int x = (int)((__float_as_uint(big) >> 23) & 255) - 126; // 2^x > big
-                ed = (float)x, edlim = __int_as_float((x + 127) << 23);
+                const int x = (int)((__float_as_uint(big) >> 23) & 255) - 126, was = ed; // 2^x > big
+                ed = x > -8 ? max(x, 0) : x;
+                edlim = __int_as_float((ed + 127) << 23);
+                if (was < 0) units = __int_as_float((was - min(ed, 0) + 127) << 23);
             }
 #pragma unroll
             for (int r = 0; r < NT; r++) {
@@ -838,12 +846,13 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
                     for (int x = 4; x <= 16; x <<= 1) f[r][i] = fmaxf(f[r][i], __shfl_xor_sync(0xffffffffu, f[r][i], x));
                     top[r][i] = fmaxf(top[r][i], f[r][i]);
-                    const float to = top[r][i] == NONE ? NONE : __fadd_ru(top[r][i], ed - TOP);
+                    const float to = top[r][i] == NONE ? NONE : __fadd_ru(top[r][i], (float)max(ed, 0) - TOP);
                     f[r][i] = ref[r][i] == to ? 1.0f : trx_a4_exp2(ref[r][i] - to);
                     ref[r][i] = to;
                 }
 #pragma unroll
                 for (int i = 0; i < 4; i++) accm[r][i] *= f[r][i & 1];
+                f[r][0] *= units, f[r][1] *= units;
 #pragma unroll
                 for (int g = 0; g < NG; g++)
 #pragma unroll
@@ -851,6 +860,15 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
                         for (int i = 0; i < 4; i++) acc[g][h][r][i] *= f[r][i & 1];
             }
+        }
+        float mid = (float)MID;
+        if (ed < 0) { // (the record is this warp's until it is fetched over)
+#pragma unroll
+            for (int k = 0; k < NG / 2; k++)
+                *reinterpret_cast<uint32_t *>(rec + L::VD + lane * (NG * 2) + 4 * k) =
+                    trx_a4_hmul2(vd[k], (uint32_t)(15 - ed) * 0x04000400u);
+            mid = __int_as_float((ed + 127) << 23) * (float)MID;
+            __syncwarp();
         }
         uint32_t ps[4][NT], pls[4]; // 8 positions each
 #pragma unroll
@@ -883,7 +901,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 if constexpr (MID != 0) {
                     const uint32_t x = n < NG ? *reinterpret_cast<const uint32_t *>(rec + L::VD + (8 * t + 4 * k + cc) * (NG * 4) + n * 4) : 0u;
                     const float2 md = trx_a4_float2(m[k]), dd = trx_a4_float2(MASK ? trx_a4_finite(x) : x);
-                    const float y = __fmaf_rn(dd.x, (float)MID, md.x), z = __fmaf_rn(dd.y, (float)MID, md.y);
+                    const float y = __fmaf_rn(dd.x, mid, md.x), z = __fmaf_rn(dd.y, mid, md.y);
                     m[k] = trx_a4_half2(y * 0.0625f, z * 0.0625f);
                     const float2 r = trx_a4_float2(m[k]);
                     ml[k] = trx_a4_half2(__fmaf_rn(r.x, -16.0f, y), __fmaf_rn(r.y, -16.0f, z));
@@ -948,7 +966,8 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
 #pragma unroll
                 for (int g = 0; g < NG; g++) { // dims 32 g + 4 n + 0..3
                     const float m = __shfl_sync(0xffffffffu, own, 4 * g + cc);
-                    const float e = EXACT ? 1.0f : 16777216.0f, f = EXACT ? 1.0f : 1048576.0f; // 2^24, 2^20
+                    const float x = __int_as_float((min(ed, 0) + 127) << 23);
+                    const float e = (EXACT ? 1.0f : 16777216.0f) * x, f = (EXACT ? 1.0f : 1048576.0f) * x; // 2^24, 2^20
                     *reinterpret_cast<float4 *>(o + row * HD + 32 * g + 4 * n) =
                         make_float4(__fmaf_rn(acc[g][0][r][i], e, m), __fmaf_rn(acc[g][0][r][2 + i], f, m),
                                     __fmaf_rn(acc[g][1][r][i], e, m), __fmaf_rn(acc[g][1][r][2 + i], f, m));
