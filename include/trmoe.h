@@ -311,10 +311,13 @@ TRMOE_API int tr_gpu_attn_warm(tr_gpu_attn *a, uint64_t ns);
  * The device calls enqueue on `stream` (a cudaStream_t; NULL: the default stream), never wait and allocate nothing, so a
  * CUDA graph can hold them. They share no workspace: calls of one session may overlap on several streams as long as
  * none writes what another one of them reads or writes (the caller orders those). Each makes the session's device
- * current on the calling thread; every pointer is memory of that device, rows of `type` (TRMOE_F32, TRMOE_F16 or
- * TRMOE_BF16), a row's heads side by side, strides in values between rows; rows start on 16-byte boundaries (the
- * stride too); an output's rows overlap neither each other nor an input. 0, or -1 with trmoe_last_error(). */
+ * current on the calling thread; every pointer is memory of that device (others are refused), rows of `type` (TRMOE_F32,
+ * TRMOE_F16 or TRMOE_BF16), a row's heads side by side, strides in values between rows; rows start on 16-byte boundaries
+ * (the stride too); an output's rows overlap neither each other nor an input. 0, or -1 with trmoe_last_error(). */
 typedef struct tr_gpu_attn4 tr_gpu_attn4;
+/* A chosen device (CUDA's number of it) for the sessions below, as tr_gpu_open gives the first: NULL with a message when it is
+ * not there or not of compute capability 10.0. */
+TRMOE_API tr_gpu *tr_gpu_open_device(int device, char *err, size_t err_len);
 #define TRMOE_ATTN4_BLOCK 64      /* positions of a selectable block */
 #define TRMOE_ATTN4_MAX_GROUP 256 /* query heads a KV head */
 

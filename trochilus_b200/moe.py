@@ -38,7 +38,7 @@ EXPORTS = ["tr_gpu_moe_create", "tr_gpu_moe_free", "tr_gpu_moe_bytes", "tr_gpu_m
            "tr_gpu_attn_free", "tr_gpu_attn_bytes", "tr_gpu_attn_write", "tr_gpu_attn_decode", "tr_gpu_attn_warm",
            "tr_gpu_attn4_create", "tr_gpu_attn4_free", "tr_gpu_attn4_bytes", "tr_gpu_attn4_write_dev",
            "tr_gpu_attn4_read_dev", "tr_gpu_attn4_attend_dev", "tr_gpu_attn4_select_dev", "tr_gpu_attn4_check",
-           "tr_gpu_attn4_write", "tr_gpu_attn4_decode", "trmoe_kernel_arch"]
+           "tr_gpu_attn4_write", "tr_gpu_attn4_decode", "tr_gpu_open_device", "trmoe_kernel_arch"]
 
 
 class Config(C.Structure):
@@ -152,6 +152,8 @@ def lib():
     L.tr_gpu_attn_decode.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
                                      C.c_float, C.c_void_p]
     L.tr_gpu_attn_warm.argtypes = [C.c_void_p, C.c_uint64]
+    L.tr_gpu_open_device.restype = C.c_void_p
+    L.tr_gpu_open_device.argtypes = [C.c_int, C.c_char_p, C.c_size_t]
     L.tr_gpu_attn4_create.restype = C.c_void_p
     L.tr_gpu_attn4_create.argtypes = [C.c_void_p, C.POINTER(Attn4Config), C.c_char_p, C.c_size_t]
     L.tr_gpu_attn4_free.argtypes = [C.c_void_p]
@@ -460,13 +462,15 @@ class GpuAttn:
 class GpuAttn4:
     """A tr_gpu_attn4 session: n_layers layers of n_seq sequences of n_ctx positions, keys and values held in 4 bits.
     The *_dev calls take device pointers (e.g. torch tensors' data_ptr()) and an Attn4Batch, and are enqueued on
-    `stream` (0: the default stream); type is F32, F16 or BF16, strides are in values."""
+    `stream` (0: the default stream); type is F32, F16 or BF16, strides are in values. device: the GPU that holds the session
+    and every pointer (None: the first that the library's kernels run on)."""
 
-    def __init__(self, n_layers: int, n_seq: int, n_head: int, n_kv_head: int, head_dim: int, n_ctx: int):
+    def __init__(self, n_layers: int, n_seq: int, n_head: int, n_kv_head: int, head_dim: int, n_ctx: int,
+                 device: int | None = None):
         L = lib()
         self.cfg = Attn4Config(n_layers, n_seq, n_head, n_kv_head, head_dim, n_ctx)
         err = C.create_string_buffer(512)
-        self.g = L.tr_gpu_open(err, 512)
+        self.g = L.tr_gpu_open(err, 512) if device is None else L.tr_gpu_open_device(device, err, 512)
         if not self.g:
             raise RuntimeError(f"tr_gpu_open: {err.value.decode()}")
         self.a = L.tr_gpu_attn4_create(self.g, C.byref(self.cfg), err, 512)
