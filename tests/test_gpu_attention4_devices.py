@@ -1,4 +1,6 @@
 """Where the 4-bit KV cache's arrays may lie: on the session's device; host memory is refused before anything is launched."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -52,3 +54,27 @@ def test_a_chosen_device(cuda):
     assert np.array_equal(gk.cpu().numpy(), orc.held(k.numpy())) and np.array_equal(gv.cpu().numpy(), orc.held(v.numpy()))
     a.check()
     a.close()
+
+
+def test_a_refused_launch_is_its_own_call_s_error(cuda):
+    """a call on the default stream while a stream that it waits for is captured fails; the calls after it do not"""
+    torch = cuda
+    rt = C.CDLL("libcudart.so.12")
+    s = Session(torch, 1, 4, 2, 64, 130)
+    rng = np.random.default_rng(62)
+    q, out = torch.ones((1, 256), device="cuda"), torch.zeros((1, 256), device="cuda")
+    b, stream, graph = s.batch([(0, 0, 1)]), C.c_void_p(), C.c_void_p()
+    assert rt.cudaStreamCreate(C.byref(stream)) == 0
+    torch.cuda.synchronize()
+    assert rt.cudaStreamBeginCapture(stream, 2) == 0
+    L, a, F32 = s.moe.lib(), s.s.a, s.moe.F32
+    failed = L.tr_gpu_attn4_attend_dev(a, 0, b, F32, q.data_ptr(), 256, 0.1, out.data_ptr(), 256, None)
+    rt.cudaStreamEndCapture(stream, C.byref(graph))
+    rt.cudaGetLastError()
+    assert failed == -1 and "attention kernel" in s.moe.last_error()
+    s.write([(0, 0, 130)], *rng.normal(size=(2, 130, 2, 64)).astype(np.float32))  # (raises if the call fails)
+    gk, gv = s.read([(0, 0, 130)])
+    assert np.array_equal(gk, s.k[0]) and np.array_equal(gv, s.v[0])
+    s.s.check()
+    assert rt.cudaStreamDestroy(stream) == 0
+    s.close()
