@@ -220,3 +220,20 @@ def test_values_that_grow(cuda, kind):
         _check(s, [(0, at, 1), (0, at, 2)], q, kind)
         _check(s, [(0, at, 1), (0, at, 2)], q, kind, n_sel=5)
     s.close()
+
+
+def test_more_selecting_rows_than_a_launch_holds(cuda):
+    """max_rows x heads past a launch's size: refused (in 32 bits the size would wrap to a launch of one row)"""
+    ctx = (1 << 23) + 1
+    s = Session.__new__(Session)
+    from trochilus_b200 import moe
+    s.torch, s.moe, s.layer, s.heads, s.kv, s.hd, s.ctx, s.keep = cuda, moe, 0, 256, 1, 64, ctx, []
+    s.s = moe.GpuAttn4(1, 1, 256, 1, 64, ctx)
+    q, out = cuda.ones((2, 256 * 64), device="cuda"), cuda.zeros((2, 256 * 64), device="cuda")
+    for n_tok, max_rows, want in ((ctx, ctx, -1), (ctx, 1 << 22, -1), (2, ctx, 0), (2, 2, 0)):
+        b = s.batch([(0, 0, 2)], n_tok=n_tok, max_rows=max_rows)
+        rc = moe.lib().tr_gpu_attn4_select_dev(s.s.a, 0, b, moe.F32, q.data_ptr(), 256 * 64, 0.1, 2, out.data_ptr(), 256 * 64, None,
+                                               None)
+        assert rc == want and (rc == 0 or "too many" in moe.last_error())
+    s.s.check()
+    s.s.close()
