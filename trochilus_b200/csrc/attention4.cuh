@@ -1158,7 +1158,7 @@ __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
                   int list_at) {
     constexpr int N = 32 * W, PW = HD / 64; // words of bounds a lane takes of a block
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int16_t s_pn[2 * HD]; // N, then P, as the bounds
+    __shared__ __align__(16) int16_t s_pn[2 * HD]; // N, then P, as the bounds (read as words)
     __shared__ int s_hist[4][256], s_warp[2][W], s_cnt[2], s_pick[2][3], s_before[2];
     int slot, row0, rows, pos0;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kv = blockIdx.y, G = a.n_head / a.n_kv;
