@@ -72,6 +72,9 @@ def test_a_refused_launch_is_its_own_call_s_error(cuda):
     rt.cudaStreamEndCapture(stream, C.byref(graph))
     rt.cudaGetLastError()
     assert failed == -1 and "attention kernel" in s.moe.last_error()
+    f = s.moe.GpuAttn(1, 2, 64)  # (another part of the library, which asks for the last error after its launches)
+    f.write(0, 0, *rng.normal(size=(2, 3, 2, 128)).astype(np.float32))
+    f.close()
     s.write([(0, 0, 130)], *rng.normal(size=(2, 130, 2, 64)).astype(np.float32))  # (raises if the call fails)
     gk, gv = s.read([(0, 0, 130)])
     assert np.array_equal(gk, s.k[0]) and np.array_equal(gv, s.v[0])

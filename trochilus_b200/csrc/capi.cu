@@ -56,6 +56,7 @@ void put_err(char *err, size_t err_len) {
 
 bool ck(cudaError_t e, const char *what) {
     if (e == cudaSuccess) return true;
+    cudaGetLastError(); // (reported here: the next launch, which asks for the last error, must not find it)
     set_err("%s: %s", what, cudaGetErrorString(e));
     return false;
 }
