@@ -338,7 +338,9 @@ typedef struct {
 typedef struct {
     int64_t n_entries;    /* <= 65535 */
     int64_t n_tok;        /* rows of the call's arrays */
-    int64_t max_rows;     /* at least the most rows of an entry (at most n_ctx); sizes the launch. Not read without start */
+    int64_t max_rows;     /* at least the most rows of an entry (at most n_ctx): sizes the launch, and an attention call of
+                           * 16-bit rows takes the kernel for many rows by it, which entries of few rows are slower in.
+                           * Not read without start */
     const int32_t *slot;  /* [n_entries] */
     const int32_t *pos0;  /* [n_entries] */
     const int32_t *start; /* [n_entries + 1], or NULL: one row an entry (n_tok = n_entries) */
@@ -364,8 +366,12 @@ TRMOE_API int tr_gpu_attn4_read_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu
 /* out row = softmax(scale q.k) v over positions 0 .. p of the row's sequence, p the row's own position (whose key and
  * value a write has stored before, as all positions before it): one row an entry is a decode step, several are a prompt
  * or drafted tokens. q and out [n_tok][n_head * head_dim]. Scores and sums are in 32 bits, and so is the rest for f32
- * rows (two 16-bit parts of each factor); for 16-bit rows a probability is rounded to f16 (2^-12 relative), and in calls
- * of many rows the keys and values are. A NaN or an infinity among the positions that a row sees makes that head's
+ * rows (two 16-bit parts of each factor). For 16-bit rows a probability and its product with a value's scale are rounded
+ * to f16 (2^-11 relative), and in calls of many rows the probability, the keys and the values are: f16 outputs are 6.5e-4
+ * off in norm at 131,000 positions of random values (their own rounding: 2e-4), bf16 ones no more than their rounding.
+ * f16 holds products down to 2^-32 of the largest weight times the largest scale of the KV head (or 1, between scales of
+ * 2^-8 and 1): where a group holds values of 6e4 and one position has 2^18 times the others' weight, what the others add to
+ * the other groups can be 2.5e-2 off. A NaN or an infinity among the positions that a row sees makes that head's
  * output, or its group of 32 values, NaN; among others it does not matter. One in a head's q makes that head's output
  * NaN, one as scale every output. */
 TRMOE_API int tr_gpu_attn4_attend_dev(tr_gpu_attn4 *a, int64_t layer, const tr_gpu_attn4_batch *batch, int type,
@@ -373,8 +379,8 @@ TRMOE_API int tr_gpu_attn4_attend_dev(tr_gpu_attn4 *a, int64_t layer, const tr_g
                                       void *stream);
 /* tr_gpu_attn4_attend_dev over n_blocks blocks of TRMOE_ATTN4_BLOCK positions (1 to 4096) for each row and KV head: the
  * block of the row's own position, up to it, and the n_blocks - 1 earlier ones of the highest score, ties to the lowest
- * index (all of them when there are no more). A block's score is an upper bound of its keys' summed q.k over the KV
- * head's query heads, in whole numbers: f32(sum_i P_i hi_i + N_i lo_i) * unit, where
+ * index (all of them when there are no more). A block's score is what its keys' summed q.k over the KV head's query heads
+ * can reach, up to the rounding of q and of the bounds, in whole numbers: f32(sum_i P_i hi_i + N_i lo_i) * unit, where
  *   unit = 2^(e-7) with 2^(e-1) <= the largest |value| of the block's 64 keys < 2^e (2^-7 where that is 0), and
  *   lo_i, hi_i = floor and ceil of dim i's lowest and highest value / unit, within -127 .. 127;
  *   P_i, N_i = the sums over the query heads of max(z, 0) and min(z, 0), z = rint(q_i / u) within -127 .. 127, and u

@@ -4,7 +4,7 @@
 // A row is one position's key or value of one KV head (HD = 64 or 128 values) in groups of 32 consecutive values. A
 // group holds a scale d and a minimum m (both f16) and a code 0..15 a value; a value reads back as f32(m + d code):
 //   m = f16(min),  d = f16(max(0, max - m) / 15),  code = clamp(rint((x - m) / d), 0, 15), 0 where d is 0.
-// Every rounding is of the real quotient (trx_a4_quant decides a quotient next to a border in 64 bits), so the codes do
+// Every rounding is of the real quotient (trx_a4_quant decides a quotient next to a border exactly), so the codes do
 // not depend on how they are computed. A group that holds a NaN or an infinity, or whose m or d passes f16, keeps
 // d = NaN, m = 0 and codes 0: it reads back as NaN, and m is always finite.
 //
@@ -458,9 +458,9 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 //            parts
 //   softmax  a reference a row, which moves only when a score passes it (16-bit rows: by 2^8), so that the usual record
 //            needs one vote and no reduction; p in f16 (f32 rows: two f16 parts, 22 bits), transposed in registers (movmatrix).
-//            16-bit rows' p, p d and subnormal codes leave f16 outputs 6e-4 off 64 bits at 100,000 positions of random values,
-//            whose outputs' own rounding is 2e-4 (bf16: 1.7e-3, all of it the outputs'); codes as integers 3.4e-4, for a third
-//            more time
+//            16-bit rows' p, p d and subnormal codes leave f16 outputs 6.5e-4 off 64 bits at 131,000 positions of random values,
+//            whose outputs' own rounding is 2e-4 (bf16: 1.6e-3, nearly all of it the outputs'); codes as integers 3.4e-4 at
+//            100,000, for a third more time
 //   outputs  mma m16n8k16: A = 16 dims x 16 positions of codes, B = p_t d_tg of 8 rows; one more with the minima (and
 //            ones, which sum p) as A.
 // 16 query rows of f16 or bf16 type, or 8 (R), share the codes' unpacking; scores, sums and outputs are f32.
@@ -473,9 +473,9 @@ __global__ void __launch_bounds__(256) trx_a4_read(TrxA4 a, TrxA4Batch b, T *__r
 // CTA through shared memory, and the CTAs' through distributed shared memory, so that no workspace or second launch is
 // needed and overlapping calls share nothing.
 //
-// What bounds it: HBM where the CTAs fill the GPU (64 sequences of 8192 positions, 32 heads over 8 of 128, bf16: 117 us, 5.7
-// TB/s, 0.87 of the measured copy rate); a record's 449 warp instructions where clusters leave SMs idle (one such sequence of
-// 131,072 positions: 46.7 us, 3.6 TB/s on 80 SMs) or many rows share the records (f32 prompts).
+// What bounds it: HBM where the CTAs fill the GPU (64 sequences of 8192 positions, 32 heads over 8 of 128, bf16: 115 us, 5.8
+// TB/s, 0.89 of the measured copy rate); a record's 454 warp instructions where clusters leave SMs idle (one such sequence of
+// 131,072 positions: 47.5 us, 3.5 TB/s on 80 SMs) or many rows share the records (f32 prompts).
 #define TRX_A4_STAGES 2
 
 __device__ __forceinline__ void trx_a4_mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -932,7 +932,7 @@ template <int HD, bool F32, int R> struct TrxA4Warp {
                 for (int r = 0; r < NT; r++) {
                     uint32_t b0 = trx_a4_hmul2(p[0][r], d[0][g]), b1 = trx_a4_hmul2(p[1][r], d[1][g]);
                     // (f32: 16 positions from 0, then added with rounding: the tensor core's additions to a sum do not round,
-                    // and 131,072 positions of 8 KV heads were 7.6e-6 off 64 bits, now 8.6e-7, for 6 to 8 % of the time.
+                    // and 131,072 positions of 8 KV heads were 7.6e-6 off 64 bits, now about 1e-6, for 6 to 8 % of the time.
                     // 16-bit rows: no change beside their roundings of p)
                     float y[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
                     float(&o0)[4] = F32 ? y[0] : acc[g][0][r], (&o1)[4] = F32 ? y[1] : acc[g][1][r];
@@ -1138,8 +1138,8 @@ __device__ __forceinline__ uint32_t trx_a4_key(float f) {
 }
 
 // Attention to n_sel blocks: the row's own and the n_sel - 1 earlier ones of the best scores (ties to the lowest
-// index). A block's score is f32(sum_i P_i highest_i + N_i lowest_i) x unit, an upper bound of the group's summed q.k
-// in whole numbers: P_i and N_i sum the positive and the negative parts of the group's query values, which are rounded
+// index). A block's score is f32(sum_i P_i highest_i + N_i lowest_i) x unit, what the group's summed q.k can reach (up to
+// the roundings) in whole numbers: P_i and N_i sum the positive and the negative parts of the group's query values, which are rounded
 // to multiples of a power of two that puts the largest magnitude in [64, 128) and kept within 127. Sums of whole
 // numbers do not depend on their order, so neither does the selection. A block with a NaN among its keys scores +inf;
 // a query with one selects by index. blocks (optional): the selected blocks, ascending, then -1.
@@ -1149,9 +1149,9 @@ __device__ __forceinline__ uint32_t trx_a4_key(float f) {
 // histograms; each CTA sends its selected blocks to every CTA's list, and the cluster attends to the list.
 // blockIdx.x = (row x tiles of R heads) x CTA of the cluster, y the KV head, z the entry. Dynamic shared memory: the
 // tile's (the keys take its place before it starts), at least keys x 4 bytes, then n_sel ints (list_at).
-// What bounds it: latency. 24 x 4 rows, 16 of up to 512 blocks, 16 heads of 64 over 4, f32: 35 us in 1.3 rounds of CTAs, of
+// What bounds it: latency. 24 x 4 rows, 16 of up to 512 blocks, 16 heads of 64 over 4, f32: 36 us in 1.3 rounds of CTAs, of
 // whose 34,500 cycles 10 % load the queries, 24 % score, 16 % find the threshold, 5 % make the list, 45 % attend. One row,
-// 32 of 2047 blocks, 32 heads over 8 of 128, bf16: 17 us (all positions 47).
+// 32 of 2047 blocks, 32 heads over 8 of 128, bf16: 17 us (all positions 48).
 template <int HD, bool F32, int R, int W>
 __global__ void __launch_bounds__(32 * W, R == 8 ? 16 / W : 1)
     trx_a4_select(TrxA4 a, TrxA4Batch b, TrxA4Rows io, float scale, int n_sel, int32_t *__restrict__ blocks, int ranks,

@@ -15,14 +15,14 @@
 //                the warp's rows move up and O, P and the sums so far are rescaled (p stays below 2^15)
 // What bounds it: each tile's own chain, a softmax pass (2200 to 2800 cycles for 128 positions) and then its products (P V
 // 1000, the next Q K^T 550, with the waits between), 4800 cycles of which the other tile's softmax covers half; converting
-// the records takes 3000 of the same cycles in other warps. 2 x 2048 rows of 32 heads at the end of 4096 positions: 291 us,
-// 0.43 of the measured bf16 rate; 8192 rows from the first position 694 us, 0.48. The loops are kept short: with all of them
+// the records takes 3000 of the same cycles in other warps. 2 x 2048 rows of 32 heads at the end of 4096 positions: 292 us,
+// 0.43 of the measured bf16 rate; 8192 rows from the first position 696 us, 0.48. The loops are kept short: with all of them
 // unrolled the warps waited for instructions (480 us). Scores in two halves of 64 positions, the first of which need not wait
 // for P V: 310 us (products with N = 64 read the queries twice).
 // Tensor memory: S 0, S 1, O 0, O 1, 128 columns each (O: HD).
 //
-// The keys' and values' rounding to f16 (2^-12 relative) is the choice that the 16-bit rows allow: half a step of f16
-// rows, a sixteenth of bf16's. Values past f16 (|m| + 15 d > 60000, which a cache of bf16 or f32 rows may hold) make the
+// The keys' and values' rounding to f16 (2^-11 relative at most) is the choice that the 16-bit rows allow: half a step of
+// f16 rows, a sixteenth of bf16's. Values past f16 (|m| + 15 d > 60000, which a cache of bf16 or f32 rows may hold) make the
 // CTA start again with all keys and all values multiplied by a power of two that fits the largest of its context.
 // Scores of 2^22 and more (log2) make it start again too, with each product of a score and its factor rounded as the
 // maximum's is: what a fused one keeps beside the reference would let p pass f16 from 2^24 on. (Rounding them always: 309 us
